@@ -260,6 +260,41 @@ int64_t bcfft_grad_c_workspace_bytes(int64_t n_tokens, int in_features, int out_
 int bcfft_grad_c(const void* x, int x_dtype, const void* dy, int dy_dtype, int64_t n_tokens, int in_features,
                  int out_features, int block_size, void* workspace, void* dc, int dc_dtype, void* stream);
 
+/* A teacher's top logits: for each of n_rows rows of `vocab` logits (row_stride elements apart) the k
+ * largest, in descending order (equal logits: the lower index first; NaN before everything), their
+ * indices, and rest = log(sum of exp(logit / temperature) over all the others) (-inf: none left). The
+ * compressed form of the teacher cache that calibrate_bc.py:192-212 keeps as whole rows of logits.
+ *   logits: dtype, element-aligned; values: (n_rows, k) of dtype; indices: (n_rows, k); rest: (n_rows)
+ *   1 <= k <= min(vocab, 1024). One launch; the outputs do not depend on scheduling. */
+int bcfft_topk_logits(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride, int k,
+                      double temperature, void* values, int32_t* indices, float* rest, void* stream);
+
+/* Distillation from a teacher's top logits: the loss KL(P || q) of bench_all_in_one.py:112-120 /
+ * calibrate_bc.py:281-294 with P the teacher's distribution over its k entries and, with `rest`, over
+ * "any other token" as one more entry, and q the student's softmax of logits / temperature:
+ *   loss[n] = weight[n] * (sum_j P_j (log P_j - log q_{i_j}) + P_rest (log P_rest - log q_rest))
+ * Without rest P is renormalised over the entries. No factor temperature^2.
+ *   values / indices: (n_rows, k), values of values_dtype, indices of index_bytes (4 or 8); an index
+ *     outside [0, vocab) marks no entry; the same index twice adds up; 1 <= k <= 1024
+ *   rest: (n_rows) as bcfft_topk_logits gives it for the same temperature, or NULL
+ *   weight: (n_rows) or NULL (1); a row of weight 0, or without an entry of any mass, has loss 0 and
+ *     gradient 0 whatever its logits hold
+ *   loss: (n_rows); stats: (n_rows, 4), 16-B aligned, for bcfft_distill_topk_backward, or NULL
+ *   grad: (n_rows, vocab) of dtype, contiguous: the gradient of the SUM of all losses with respect to
+ *     the logits, or NULL. With it the row is read once for both.
+ * vocab <= 262144. -inf logits are masked tokens; where the teacher gives one mass the loss is +inf and
+ * the gradient q - P. Sums in fp32 per thread, fp64 across threads; deterministic. */
+int bcfft_distill_topk(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                       const void* values, int values_dtype, const void* indices, int index_bytes, int k,
+                       const float* rest, const float* weight, double temperature, float* loss, float* stats,
+                       void* grad, void* stream);
+
+/* grad[n] = upstream[n] * dloss[n]/dlogits[n] from the forward's stats and the same operands. */
+int bcfft_distill_topk_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                                const void* values, int values_dtype, const void* indices, int index_bytes, int k,
+                                const float* rest, const float* weight, double temperature, const float* stats,
+                                const float* upstream, void* grad, void* stream);
+
 /* Single circulant matvec y = C(c) x, C[i,j] = c[(i-j) mod n], any n >= 1.
  * Replaces fft_utils.circulant_matvec_fft (fft_utils.py:3-34); c, x, y share `dtype`.
  * Direct O(n^2) evaluation accumulated in fp64 (this entry point serves validation-sized

@@ -4,6 +4,7 @@ The teacher/student metrics and batching of src/bench_all_in_one.py, restated ov
   * pad_batch / iter_batches      bench_all_in_one.py:79-101 (right padding, last real index)
   * gather_last_logits            bench_all_in_one.py:103-110
   * softmax_kl                    bench_all_in_one.py:112-120 (KL(teacher || student), per row)
+  * teacher_cache, distill_kl     calibrate_bc.py:192-212, 281-294 (KL from the teacher's top logits, on the GPU)
   * last_token_metrics            bench_all_in_one.py:295-345 (same keys; the reference loops
                                   one prompt at a time, here a batch of rows is scored at once
                                   with the same per-row formulas and averaged the same way)
@@ -72,6 +73,25 @@ def softmax_kl(student: torch.Tensor, teacher: torch.Tensor, temperature: float 
     log_p = torch.log_softmax(teacher / t, dim=-1)
     log_q = torch.log_softmax(student / t, dim=-1)
     return (log_p.exp() * (log_p - log_q)).sum(dim=-1)
+
+
+def teacher_cache(logits: torch.Tensor, k: int = 64, temperature: float = 1.0) -> Dict[str, object]:
+    """A teacher's rows of logits (..., V) as distill_kl takes them: the k largest, their indices and
+    the log of the mass outside them, instead of the whole rows that calibrate_bc.py:192-212 keeps
+    (LLaMA-2's 32000 bf16 logits: 64 KB a row; k = 64: 388 B). ROCm tensors only."""
+    from bcfft import distill
+    values, indices, rest = distill.topk_logits(logits, k, temperature)
+    return {"values": values, "indices": indices, "rest": rest, "temperature": float(temperature)}
+
+
+def distill_kl(student: torch.Tensor, cache: Dict[str, object], weight: torch.Tensor | None = None) -> torch.Tensor:
+    """KL(teacher || student) per row from a teacher_cache, differentiable in student: softmax_kl of the
+    two distributions after every token outside the cached ones is merged into one outcome (at
+    k = V it is softmax_kl itself). The calibration loss of calibrate_bc.py:281-294; its mean over
+    rows is distill_kl(...).mean(). ROCm tensors only."""
+    from bcfft import distill
+    return distill.topk_kl(student, cache["values"], cache["indices"], rest=cache["rest"], weight=weight,
+                           temperature=cache["temperature"])
 
 
 def last_token_metrics(student: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0,

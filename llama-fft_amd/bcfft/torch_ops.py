@@ -10,12 +10,15 @@ a host tensor fails loudly as in bcfft.ops.
     torch.ops.bcfft.spectra(c, transpose_conj) -> spec
     torch.ops.bcfft.forward_glu(x2d, spec_gu, block_size, gate_features, algo) -> h
     torch.ops.bcfft.forward_mlp(x2d, spec_gu, spec_down, block_size, inter_features, mode) -> y
+    torch.ops.bcfft.topk_logits(logits, k, temperature) -> values, indices, rest
+    torch.ops.bcfft.topk_kl(logits, values, indices, rest, weight, temperature) -> loss (forward only)
+    torch.ops.bcfft.topk_kl_grad(...) -> loss, dlogits
 """
 from __future__ import annotations
 
 import torch
 
-from . import _lib, ops
+from . import _lib, distill, ops
 
 
 @torch.library.custom_op("bcfft::forward", mutates_args=())
@@ -81,9 +84,53 @@ def _forward_mlp_fake(x2d, spec_gu, spec_down, block_size, inter_features, mode=
     return x2d.new_empty(x2d.shape)
 
 
+@torch.library.custom_op("bcfft::topk_logits", mutates_args=())
+def topk_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A teacher's k largest logits, indices and rest: bcfft.distill.topk_logits (calibrate_bc.py:192-212)."""
+    return distill.topk_logits(logits, k, temperature)
+
+
+@topk_logits.register_fake
+def _topk_logits_fake(logits, k, temperature=1.0):
+    if logits.dim() < 1 or not 1 <= k <= logits.shape[-1]:
+        raise ValueError("bcfft::topk_logits: logits must be (..., V) with 1 <= k <= V")
+    lead = logits.shape[:-1]
+    return (logits.new_empty((*lead, k)), logits.new_empty((*lead, k), dtype=torch.int32),
+            logits.new_empty(lead, dtype=torch.float32))
+
+
+@torch.library.custom_op("bcfft::topk_kl", mutates_args=())
+def topk_kl(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, rest: torch.Tensor | None = None,
+            weight: torch.Tensor | None = None, temperature: float = 1.0) -> torch.Tensor:
+    """KL per row from the teacher's top logits: bcfft.distill.topk_kl's forward (calibrate_bc.py:281-294)."""
+    return distill.topk_kl(logits.detach(), values, indices, rest=rest, weight=weight, temperature=temperature)
+
+
+@topk_kl.register_fake
+def _topk_kl_fake(logits, values, indices, rest=None, weight=None, temperature=1.0):
+    if values.shape != indices.shape or values.shape[:-1] != logits.shape[:-1]:
+        raise ValueError("bcfft::topk_kl: values and indices must both be logits' leading shape + (k,)")
+    return logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.custom_op("bcfft::topk_kl_grad", mutates_args=())
+def topk_kl_grad(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, rest: torch.Tensor | None = None,
+                 weight: torch.Tensor | None = None, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Losses and the gradient of their sum in one launch: bcfft.distill.topk_kl_grad."""
+    return distill.topk_kl_grad(logits.detach(), values, indices, rest=rest, weight=weight, temperature=temperature)
+
+
+@topk_kl_grad.register_fake
+def _topk_kl_grad_fake(logits, values, indices, rest=None, weight=None, temperature=1.0):
+    return (_topk_kl_fake(logits, values, indices, rest, weight, temperature),
+            torch.empty(logits.shape, dtype=logits.dtype, device=logits.device))
+
+
 def registered() -> bool:
     """True once the ops are visible under torch.ops.bcfft (importing this module registers them)."""
-    return all(hasattr(torch.ops.bcfft, n) for n in ("forward", "spectra", "forward_glu", "forward_mlp"))
+    return all(hasattr(torch.ops.bcfft, n) for n in ("forward", "spectra", "forward_glu", "forward_mlp",
+                                                          "topk_logits", "topk_kl", "topk_kl_grad"))
 
 
-__all__ = ["forward", "spectra", "forward_glu", "forward_mlp", "registered", "_lib"]
+__all__ = ["forward", "spectra", "forward_glu", "forward_mlp", "topk_logits", "topk_kl", "topk_kl_grad",
+           "registered", "_lib"]

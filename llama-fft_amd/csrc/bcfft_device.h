@@ -667,6 +667,8 @@ void launch_mlp_dmm_split(const void* x, int64_t n, int n_h, const void* spec_gu
 
 // weight prep (bcfft_prep.hip): loss-aware circulant projection of a dense (n_out*b, n_in*b)
 // weight into c (n_out, n_in, b) fp32; false for an unsupported block size
+// BCFFT_OK, or BCFFT_ERR_HIP with the text kept for bcfft_last_hip_error (bcfft_kernels.hip)
+int record_launch_status();
 bool launch_project(int b, const void* w, int dt, int n_out, int n_in, float eps, float* c, hipStream_t s);
 
 // dc of the BC forward (bcfft_grad.hip): token split and workspace of the two-launch reduction

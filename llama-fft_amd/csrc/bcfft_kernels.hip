@@ -716,6 +716,8 @@ void launch_spectra(const void* c, int c_dt, int n_out, int n_in, int tc, float2
 }
 }  // namespace
 
+int bcfft::record_launch_status() { return record_launch(); }
+
 extern "C" {
 
 int bcfft_abi_version(void) { return BCFFT_ABI_VERSION; }
