@@ -295,6 +295,50 @@ int bcfft_distill_topk_backward(const void* logits, int dtype, int64_t n_rows, i
                                 const float* rest, const float* weight, double temperature, const float* stats,
                                 const float* upstream, void* grad, void* stream);
 
+/* The dense projections that a partly patched model keeps (patch_llama_fft.py:343-394 replaces the
+ * projections of some layers; by default 31 of 32 MLPs stay dense).
+ *   linear: y = act(x w^T + bias) + residual          glu: h = act(x w_gate^T) * (x w_up^T)
+ * x (n_tokens, in_features) with x_stride elements between rows; w, w_gate, w_up (out_features,
+ * in_features) contiguous; bias (out_features) or NULL; residual (n_tokens, out_features) with r_stride, or
+ * NULL; y / h (n_tokens, out_features) contiguous. Everything of one dtype, element-aligned: rows that start
+ * on 16 bytes run the direct-to-LDS kernels. Products accumulate in fp32, bias, activation and residual are
+ * applied there, one rounding to dtype. Features and strides up to 2^20 (the glu backward: 2 out_features), up to 2^23
+ * tokens; n_tokens == 0 is a no-op.
+ *   z / gu: fp32, what the backward needs: x w^T + bias (n_tokens, out_features), or g then u
+ *     (2, n_tokens, out_features); NULL where there is no backward (linear: also without activation).
+ * workspace: bcfft_dense_workspace_bytes(op, ...) bytes, 16-B aligned: partial sums of products whose k is
+ *   split over workgroups, added in a fixed order (deterministic); the forwards run unsplit without it.
+ * GELU is the exact form, z * Phi(z). */
+enum bcfft_act { BCFFT_ACT_NONE = 0, BCFFT_ACT_RELU = 1, BCFFT_ACT_SILU = 2, BCFFT_ACT_GELU = 3 };
+enum bcfft_dense_op { BCFFT_DENSE_LINEAR = 0, BCFFT_DENSE_GLU = 1, BCFFT_DENSE_LINEAR_BACKWARD = 2,
+                      BCFFT_DENSE_GLU_BACKWARD = 3 };
+
+int64_t bcfft_dense_workspace_bytes(int op, int64_t n_tokens, int64_t in_features, int64_t out_features, int dtype,
+                                    int act);
+
+int bcfft_dense_linear(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
+                       int64_t out_features, const void* w, const void* bias, const void* residual, int64_t r_stride,
+                       int act, void* y, float* z, void* workspace, int64_t workspace_bytes, void* stream);
+
+int bcfft_dense_glu(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
+                    int64_t out_features, const void* w_gate, const void* w_up, int act, void* h, float* gu,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients of linear: dz = dy act'(z) (rounded once to dtype where there is an activation), dx = dz w,
+ * dw = dz^T x, db = the columns' sums of the unrounded dz (the residual's gradient is dy itself). dx, dw, db:
+ * contiguous, of dtype, each may be NULL. n_tokens >= 1. */
+int bcfft_dense_linear_backward(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
+                                int64_t out_features, const void* w, const void* dy, int64_t dy_stride, const float* z,
+                                int act, void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes,
+                                void* stream);
+
+/* Gradients of glu: dg = dh u act'(g), du = dh act(g) (rounded once to dtype), dx = dg w_gate + du w_up, dw
+ * (2 out_features, in_features): w_gate's gradient above w_up's. dx, dw may be NULL. n_tokens >= 1. */
+int bcfft_dense_glu_backward(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
+                             int64_t out_features, const void* w_gate, const void* w_up, const void* dh,
+                             int64_t dh_stride, const float* gu, int act, void* dx, void* dw, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
 /* Single circulant matvec y = C(c) x, C[i,j] = c[(i-j) mod n], any n >= 1.
  * Replaces fft_utils.circulant_matvec_fft (fft_utils.py:3-34); c, x, y share `dtype`.
  * Direct O(n^2) evaluation accumulated in fp64 (this entry point serves validation-sized

@@ -2,10 +2,10 @@
 
 `bcfft.torch_ops` (the torch.library registration of the ops under torch.ops.bcfft) is imported
 on first access, so the ctypes ops stay importable on a torch without torch.library.custom_op."""
-from . import _lib, distill, graph, ops  # noqa: F401
+from . import _lib, dense, distill, graph, ops  # noqa: F401
 from ._lib import LIB_PATH, SUPPORTED_BLOCKS, load  # noqa: F401
 
-__all__ = ["ops", "graph", "distill", "torch_ops", "load", "LIB_PATH", "SUPPORTED_BLOCKS"]
+__all__ = ["ops", "graph", "dense", "distill", "torch_ops", "load", "LIB_PATH", "SUPPORTED_BLOCKS"]
 
 
 def __getattr__(name):

@@ -1,0 +1,198 @@
+// bcfft_dense.h — arguments and output stages of the dense-product kernels (bcfft_dense.hip).
+#pragma once
+#include "bcfft_device.h"
+
+namespace bcfft {
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+
+struct DenseArgs {
+  const void* a[2];                      // operand of the output's rows, per segment of k
+  const void* b[2];                      // operand of the output's columns, per segment; GLU: gate and up
+  int64_t lda, ldb;                      // elements between rows (by rows) or between k-rows (by columns)
+  int64_t k;                             // elements of k per segment
+  int64_t m, n;                          // output rows and columns (GLU: columns of h)
+  const void* bias;                      // (n) or null
+  const void* res;                       // (m, n) with stride ldr, or null
+  int64_t ldr;
+  void* y;                               // (m, n) contiguous
+  float* z;                              // what the backward needs: x W^T + b (m, n); GLU: g then u (2, m, n); or null
+  float* ws;                             // (kz, m, n or 2 n) partial sums
+  int segs, kz, act;
+};
+
+struct DzArgs {
+  const void* dy;
+  int64_t ldd;
+  const float* z;                        // pre-activation, or g and u
+  void* dz;                              // dz, or rows of dg, du
+  float* part;                           // column sums per slice of rows, or null
+  int64_t m, n;
+  int act;
+};
+
+// 16 bytes at an address aligned to the element only (gfx950 serves unaligned global accesses)
+template <int E>
+struct __attribute__((packed, aligned(E))) Unaligned16 {
+  uint32_t w[4];
+};
+template <int E>
+struct __attribute__((packed, aligned(E))) Unaligned8 {
+  uint32_t w[2];
+};
+
+// elements k .. of a row of kend elements, 16 bytes, zero past the end
+template <int E>
+__device__ __forceinline__ uint4 load_part(const char* row, int64_t k, int64_t kend) {
+  constexpr int EPC = 16 / E;
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (k + EPC <= kend) {
+    const Unaligned16<E> u = *reinterpret_cast<const Unaligned16<E>*>(row + k * E);
+    return make_uint4(u.w[0], u.w[1], u.w[2], u.w[3]);
+  }
+#pragma unroll
+  for (int j = 0; j < EPC - 1; ++j) {
+    if (k + j < kend) {
+      if constexpr (E == 4) w[j] = ((const uint32_t*)row)[k + j];
+      else w[j / 2] |= (uint32_t)((const uint16_t*)row)[k + j] << 16 * (j & 1);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// elements i .. i + cnt (cnt <= 4) of an array of DT as fp32, 0 past cnt
+template <int DT>
+__device__ __forceinline__ void load4_at(const void* p, int64_t i, int cnt, float (&v)[4]) {
+  if (cnt == 4) {
+    if constexpr (DT == BCFFT_F32) {
+      const Unaligned16<4> u = *reinterpret_cast<const Unaligned16<4>*>((const float*)p + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(u.w[j]);
+    } else {
+      const Unaligned8<2> u = *reinterpret_cast<const Unaligned8<2>*>((const uint16_t*)p + i);
+      const float2 a = unpack16<DT>(u.w[0]), b = unpack16<DT>(u.w[1]);
+      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < cnt ? load_scalar(p, i + j, DT) : 0.f;
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store4_at(void* p, int64_t i, int cnt, const float (&v)[4]) {
+  if constexpr (DT == BCFFT_F32) {
+    if (cnt == 4) {
+      Unaligned16<4> u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u.w[j] = __float_as_uint(v[j]);
+      *reinterpret_cast<Unaligned16<4>*>((float*)p + i) = u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cnt) ((float*)p)[i + j] = v[j];
+    }
+  } else {
+    Unaligned8<2> u;
+    u.w[0] = pack16<DT>(v[0], v[1]);
+    u.w[1] = pack16<DT>(v[2], v[3]);
+    if (cnt == 4) {
+      *reinterpret_cast<Unaligned8<2>*>((uint16_t*)p + i) = u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cnt) ((uint16_t*)p)[i + j] = (uint16_t)(u.w[j / 2] >> 16 * (j & 1));
+    }
+  }
+}
+
+// ------------------------------------------------------------------ activations (fp32)
+// gelu is z times the normal distribution function, 0.5 erfc(-z / sqrt 2): no cancellation for z < 0
+__device__ __forceinline__ float act_value(int act, float z) {
+  switch (act) {
+    case BCFFT_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
+    case BCFFT_ACT_SILU: return silu(z);
+    case BCFFT_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);
+    default: return z;
+  }
+}
+// act(z) and act'(z)
+__device__ __forceinline__ void act_both(int act, float z, float& v, float& slope) {
+  switch (act) {
+    case BCFFT_ACT_RELU:
+      v = z > 0.f || z != z ? z : 0.f;
+      slope = z > 0.f ? 1.f : z != z ? z : 0.f;
+      break;
+    case BCFFT_ACT_SILU: {
+      const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+      v = z * s;
+      slope = s * (1.f + z * (1.f - s));
+      break;
+    }
+    case BCFFT_ACT_GELU: {
+      const float phi = 0.5f * erfcf(-0.70710678f * z);
+      v = z * phi;
+      slope = phi + z * 0.39894228f * __expf(-0.5f * z * z);
+      break;
+    }
+    default:
+      v = z;
+      slope = 1.f;
+  }
+}
+
+// ------------------------------------------------------------------ output stages
+// four consecutive columns n .. n + cnt of row m, accumulated in fp32; one rounding
+template <int DT>
+__device__ __forceinline__ void finish_linear(const DenseArgs& a, int64_t m, int64_t n, f32x4 acc, int cnt) {
+  float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+  if (a.bias) {
+    float b[4];
+    load4_at<DT>(a.bias, n, cnt, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += b[j];
+  }
+  if (a.z) store4_at<BCFFT_F32>(a.z, m * a.n + n, cnt, v);
+  if (a.act != BCFFT_ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = act_value(a.act, v[j]);
+  }
+  if (a.res) {
+    float r[4];
+    load4_at<DT>(a.res, m * a.ldr + n, cnt, r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += r[j];
+  }
+  store4_at<DT>(a.y, m * a.n + n, cnt, v);
+}
+template <int DT>
+__device__ __forceinline__ void finish_glu(const DenseArgs& a, int64_t m, int64_t n, f32x4 g, f32x4 u, int cnt) {
+  if (a.z) {
+    const float gv[4] = {g[0], g[1], g[2], g[3]}, uv[4] = {u[0], u[1], u[2], u[3]};
+    store4_at<BCFFT_F32>(a.z, m * a.n + n, cnt, gv);
+    store4_at<BCFFT_F32>(a.z + a.m * a.n, m * a.n + n, cnt, uv);
+  }
+  float h[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = act_value(a.act, g[j]) * u[j];
+  store4_at<DT>(a.y, m * a.n + n, cnt, h);
+}
+
+// partial sums of a slice of k: rows of 2 n for the gated form, whose `n` here counts both halves
+__device__ __forceinline__ int64_t partial_width(const DenseArgs& a) { return a.b[1] && a.segs == 1 ? 2 * a.n : a.n; }
+__device__ __forceinline__ void store_partial(const DenseArgs& a, int slice, int64_t m, int64_t n, f32x4 acc, int cnt) {
+  const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+  store4_at<BCFFT_F32>(a.ws, ((int64_t)slice * a.m + m) * partial_width(a) + n, cnt, v);
+}
+__device__ __forceinline__ f32x4 load_partials(const DenseArgs& a, int64_t m, int64_t n, int cnt) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < a.kz; ++k) {
+    float v[4];
+    load4_at<BCFFT_F32>(a.ws, ((int64_t)k * a.m + m) * partial_width(a) + n, cnt, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += v[j];
+  }
+  return s;
+}
+
+}  // namespace bcfft

@@ -1,0 +1,372 @@
+"""Dense projections on the GPU against a plain implementation in 64 bits.
+
+Tolerances, from the arithmetic, u = 2^-24 (half an fp32 step), h = eps / 2 of the dtype:
+  a product summed over K terms in fp32, in any order: rounding errors of random sign add up to at most
+  8 sqrt(K) u times the sum of the terms' magnitudes (eight standard deviations of K steps of u each);
+  the output is rounded once: h |y|, or half a step of the smallest subnormal.
+  activations: 16 u of their value and slope; an error d of their input gives at most 1.2 d (|act'|,
+  |act''| <= 1.2).
+  dz is rounded once to dtype where there is an activation: h |dz| per element, independent, so 8 h times
+  the root of the sum of (dz w)^2 in dx."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = 2.0 ** -24
+TINY = {torch.float32: 1e-37, torch.float16: 2.0 ** -25, torch.bfloat16: 1e-37}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a ROCm device"
+    import bcfft
+    bcfft.load()
+    return torch.device("cuda:0")
+
+
+def act64(z, act):
+    """act(z), act'(z) in fp64."""
+    if act is None:
+        return z, torch.ones_like(z)
+    if act == "relu":
+        return z.clamp_min(0), (z > 0).double()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    phi = torch.special.ndtr(z)
+    return z * phi, phi + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+
+
+def rand(dev, *shape, dt, seed, scale=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=dev) * scale).to(dt)
+
+
+def within(got, want, slack, extra=0.0):
+    h = torch.finfo(got.dtype).eps / 2
+    tol = h * (want.abs() + slack) + slack + TINY[got.dtype] + extra
+    off = (got.double() - want).abs()
+    assert got.shape == want.shape
+    assert bool((off <= tol).all()), f"off by {float((off - tol).max())} more than {float(tol.max())}"
+
+
+def sum_slack(a, b):
+    """a @ b's accumulation error: 8 sqrt(K) u times the magnitudes."""
+    return 8 * math.sqrt(a.shape[-1]) * U * (a.abs() @ b.abs())
+
+
+def linear64(x, w, b, r, act):
+    """y and its slack; z, its slack, and the slope."""
+    x, w = x.double(), w.double()
+    z = x @ w.t()
+    zs = sum_slack(x, w.t())
+    if b is not None:
+        z = z + b.double()
+        zs = zs + U * z.abs()
+    v, slope = act64(z, act)
+    ys = 1.2 * zs + 16 * U * v.abs()
+    y = v if r is None else v + r.double()
+    return y, ys + U * y.abs(), z, zs, slope
+
+
+def grads64(x, w, dy, slope, zs, act, dt):
+    """dx, dw, db and their slacks."""
+    x, w, dy = x.double(), w.double(), dy.double()
+    dz = dy * slope
+    err = dy.abs() * (1.2 * zs + 16 * U) if act else torch.zeros_like(dz)
+    h = torch.finfo(dt).eps / 2 if act else 0.0
+    tiny = TINY[dt] if act else 0.0
+    dx, dw, db = dz @ w, dz.t() @ x, dz.sum(0)
+    dxs = sum_slack(dz, w) + err @ w.abs() + 8 * h * torch.sqrt((dz * dz) @ (w * w)) + tiny * w.abs().sum(0)
+    dws = (sum_slack(dz.t(), x) + err.t() @ x.abs() + 8 * h * torch.sqrt((dz * dz).t() @ (x * x)) +
+           tiny * x.abs().sum(0))
+    dbs = (8 * math.sqrt(dz.shape[0]) * U * dz.abs() + err).sum(0)
+    return (dx, dxs), (dw, dws), (db, dbs)
+
+
+SIZES = [(1, 1, 1), (1, 64, 16), (2, 7, 5), (3, 72, 24), (16, 264, 130), (17, 100, 40), (32, 129, 33), (33, 64, 128),
+         (65, 200, 136), (130, 1000, 72), (257, 136, 264), (300, 65, 517)]
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("n,k,m", SIZES)
+def test_linear_forward(dev, dt, n, k, m):
+    from bcfft import dense
+    x, w = rand(dev, n, k, dt=DT[dt], seed=1), rand(dev, m, k, dt=DT[dt], seed=2, scale=k ** -0.5)
+    b, r = rand(dev, m, dt=DT[dt], seed=3), rand(dev, n, m, dt=DT[dt], seed=4)
+    for act, bias, res in ((None, None, None), ("silu", b, None), ("gelu", b, r), ("relu", None, r)):
+        y = dense.linear(x, w, bias, activation=act, residual=res)
+        want, slack, *_ = linear64(x, w, bias, res, act)
+        within(y, want, slack)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("n,k,m", SIZES)
+def test_linear_backward(dev, dt, n, k, m):
+    from bcfft import dense
+    x, w = rand(dev, n, k, dt=DT[dt], seed=5), rand(dev, m, k, dt=DT[dt], seed=6, scale=k ** -0.5)
+    b, r, dy = (rand(dev, *s, dt=DT[dt], seed=7 + i) for i, s in enumerate(((m,), (n, m), (n, m))))
+    for act, bias, res in ((None, None, None), (None, b, r), ("gelu", b, r), ("silu", None, None), ("relu", b, None)):
+        ins = [t.clone().requires_grad_() if t is not None else None for t in (x, w, bias, res)]
+        y = dense.linear(ins[0], ins[1], ins[2], activation=act, residual=ins[3])
+        want, slack, z, zs, slope = linear64(x, w, bias, res, act)
+        within(y.detach(), want, slack)
+        y.backward(dy)
+        # at a kink the slope is either side's: leave out z that rounding may move across it
+        if act == "relu":
+            near = (z.abs() <= zs)
+            assert float(near.double().mean()) < 0.01
+            if bool(near.any()):
+                continue
+        (dx, dxs), (dw, dws), (db, dbs) = grads64(x, w, dy, slope, zs, act, DT[dt])
+        within(ins[0].grad, dx, dxs)
+        within(ins[1].grad, dw, dws)
+        if bias is not None:
+            within(ins[2].grad, db, dbs)
+        if res is not None:
+            assert torch.equal(ins[3].grad, dy)
+
+
+def glu64(x, wg, wu, act):
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    g, u = x @ wg.t(), x @ wu.t()
+    gs, us = sum_slack(x, wg.t()), sum_slack(x, wu.t())
+    v, slope = act64(g, act)
+    vs = 1.2 * gs + 16 * U * v.abs()
+    h = v * u
+    return h, vs * u.abs() + us * v.abs() + vs * us + U * h.abs(), (g, gs, u, us, v, vs, slope)
+
+
+def glu_grads64(x, wg, wu, dh, parts, dt):
+    x, wg, wu, dh = x.double(), wg.double(), wu.double(), dh.double()
+    g, gs, u, us, v, vs, slope = parts
+    dg, du = dh * u * slope, dh * v
+    eg = dh.abs() * (us * 1.2 + u.abs() * (1.2 * gs + 16 * U)) + 4 * U * dg.abs()
+    eu = dh.abs() * vs + 2 * U * du.abs()
+    h = torch.finfo(dt).eps / 2
+    out = []
+    both, weights, err = torch.cat([dg, du], 1), torch.cat([wg, wu], 0), torch.cat([eg, eu], 1) + TINY[dt]
+    out.append((both @ weights, sum_slack(both, weights) + err @ weights.abs() +
+                8 * h * torch.sqrt((both * both) @ (weights * weights))))
+    for d, e in ((dg, eg), (du, eu)):
+        out.append((d.t() @ x, sum_slack(d.t(), x) + (e + TINY[dt]).t() @ x.abs() +
+                    8 * h * torch.sqrt((d * d).t() @ (x * x))))
+    return out
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("n,k,m", SIZES)
+def test_glu(dev, dt, n, k, m):
+    from bcfft import dense
+    x, dh = rand(dev, n, k, dt=DT[dt], seed=11), rand(dev, n, m, dt=DT[dt], seed=12)
+    wg, wu = (rand(dev, m, k, dt=DT[dt], seed=s, scale=k ** -0.5) for s in (13, 14))
+    for act in ("silu", "gelu", None):
+        h = dense.glu(x, wg, wu, activation=act)
+        want, slack, parts = glu64(x, wg, wu, act)
+        within(h, want, slack)
+        ins = [t.clone().requires_grad_() for t in (x, wg, wu)]
+        h2 = dense.glu(*ins, activation=act)
+        assert torch.equal(h2.detach(), h)
+        h2.backward(dh)
+        for t, (grad, gslack) in zip(ins, glu_grads64(x, wg, wu, dh, parts, DT[dt])):
+            within(t.grad, grad, gslack)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,k,m", [(4096, 136, 4096), (1700, 320, 4096), (2048, 264, 1000), (100, 4096, 4096)])
+def test_large_tiles(dev, dt, n, k, m):
+    """Sizes that run the larger tiles and the splits of k, forward and backward."""
+    from bcfft import dense
+    x, w = rand(dev, n, k, dt=DT[dt], seed=21), rand(dev, m, k, dt=DT[dt], seed=22, scale=k ** -0.5)
+    wu, dy = rand(dev, m, k, dt=DT[dt], seed=23, scale=k ** -0.5), rand(dev, n, m, dt=DT[dt], seed=24)
+    b = rand(dev, m, dt=DT[dt], seed=25)
+    ins = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = dense.linear(*ins, activation="silu")
+    want, slack, z, zs, slope = linear64(x, w, b, None, "silu")
+    within(y.detach(), want, slack)
+    y.backward(dy)
+    for t, (grad, gslack) in zip(ins, grads64(x, w, dy, slope, zs, "silu", DT[dt])):
+        within(t.grad, grad, gslack)
+    ins = [t.clone().requires_grad_() for t in (x, w, wu)]
+    h = dense.glu(*ins)
+    want, slack, parts = glu64(x, w, wu, "silu")
+    within(h.detach(), want, slack)
+    h.backward(dy)
+    for t, (grad, gslack) in zip(ins, glu_grads64(x, w, wu, dy, parts, DT[dt])):
+        within(t.grad, grad, gslack)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_strides_offsets_and_shapes(dev, dt):
+    """Operands at any element-aligned address, rows of a stride, leading dimensions, an expanded gradient."""
+    from bcfft import dense
+    base = rand(dev, 40, 301, dt=DT[dt], seed=31)
+    store = rand(dev, 50 * 96 + 3, dt=DT[dt], seed=32)
+    w = store[3:3 + 50 * 96].view(50, 96)                      # misaligned weight
+    for x in (base[:, 5:101], base[::2, :96], base[:, :288:3], base[:, :96].view(4, 10, 96), base[:1, :96].expand(7, 96),
+              base[0, :96], base[:36, :96].view(2, 18, 96).transpose(0, 1)):
+        xin, win = x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+        y = dense.linear(x, w, activation="silu")
+        want, slack, z, zs, slope = linear64(x.reshape(-1, 96), w, None, None, "silu")
+        assert y.shape == x.shape[:-1] + (50,)
+        within(y.reshape(-1, 50), want, slack)
+        dense.linear(xin, win, activation="silu").sum().backward()
+        (dx, dxs), (dw, dws), _ = grads64(x.reshape(-1, 96), w, torch.ones_like(want), slope, zs, "silu", DT[dt])
+        within(xin.grad.reshape(-1, 96), dx, dxs)
+        within(win.grad, dw, dws)
+        h = dense.glu(x, w, w)
+        want, slack, _ = glu64(x.reshape(-1, 96), w, w, "silu")
+        within(h.reshape(-1, 50), want, slack)
+    r = base[:20, 10:60]                                       # a residual with a row stride
+    y = dense.linear(base[:20, :96], w, residual=r)
+    want, slack, *_ = linear64(base[:20, :96], w, None, r, None)
+    within(y, want, slack)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_nan_and_inf_stay_in_their_rows(dev, dt):
+    """Rows past an operand's end are read as repeats of the last one and the end of k as zero: nothing
+    that lies there reaches another output."""
+    from bcfft import dense
+    for n, k, m in ((20, 100, 40), (140, 72, 150)):
+        x, w = rand(dev, n, k, dt=DT[dt], seed=41), rand(dev, m, k, dt=DT[dt], seed=42)
+        clean = dense.linear(x, w)
+        x[n - 1, k - 1] = math.nan
+        w[m - 1, 0] = math.inf
+        y = dense.linear(x, w)
+        assert bool(torch.isnan(y[n - 1]).all())
+        assert torch.equal(y[:n - 1, :m - 1], clean[:n - 1, :m - 1])
+        assert not bool(torch.isfinite(y[:, m - 1]).any())
+
+
+def test_no_rows(dev):
+    from bcfft import dense
+    x = torch.empty(0, 64, device=dev, requires_grad=True)
+    w, wu, b = (torch.randn(*s, device=dev, requires_grad=True) for s in ((32, 64), (32, 64), (32,)))
+    y = dense.linear(x, w, b, activation="gelu")
+    assert y.shape == (0, 32)
+    y.sum().backward()
+    assert x.grad.shape == (0, 64) and not bool(w.grad.any()) and not bool(b.grad.any())
+    w.grad = None
+    dense.glu(x, w, wu).sum().backward()
+    assert not bool(w.grad.any()) and not bool(wu.grad.any())
+
+
+def test_partial_gradients_and_no_grad(dev):
+    from bcfft import dense
+    x, w, b = rand(dev, 40, 64, dt=torch.bfloat16, seed=1), rand(dev, 48, 64, dt=torch.bfloat16, seed=2), rand(dev, 48, dt=torch.bfloat16, seed=3)
+    full = [t.clone().requires_grad_() for t in (x, w, b)]
+    dense.linear(*full, activation="silu").sum().backward()
+    for i in range(3):
+        part = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        dense.linear(*part, activation="silu").sum().backward()
+        assert torch.equal(part[i].grad, full[i].grad)
+        assert all(part[j].grad is None for j in range(3) if j != i)
+    r = rand(dev, 40, 48, dt=torch.bfloat16, seed=4).requires_grad_()
+    dense.linear(x, w, b, activation="silu", residual=r).sum().backward()
+    assert torch.equal(r.grad, torch.ones_like(r))
+    with torch.no_grad():
+        y = dense.linear(*full)
+    assert not y.requires_grad
+    g = [t.clone().requires_grad_() for t in (x, w, w)]
+    dense.glu(*g).sum().backward()
+    for i in range(3):
+        part = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, w, w))]
+        dense.glu(*part).sum().backward()
+        assert torch.equal(part[i].grad, g[i].grad)
+    with pytest.raises(RuntimeError):                     # no second derivatives
+        (dx,) = torch.autograd.grad(dense.linear(full[0], full[1]).sum(), full[0], create_graph=True)
+        dx.sum().backward()
+
+
+def test_gradient_against_differences(dev):
+    """Central differences of <dy, y(x + h d)> in fp32: y's error (its slack, per element, both sides) over
+    2 h, and h^2 / 6 times the third derivative along d (|act'''| <= 2, per element |dy| |d W|^3)."""
+    from bcfft import dense
+    n, k, m, h = 24, 40, 36, 0.02
+    x, w, wu = (rand(dev, *s, dt=torch.float32, seed=51 + i, scale=0.3) for i, s in enumerate(((n, k), (m, k), (m, k))))
+    dy = rand(dev, n, m, dt=torch.float32, seed=55)
+    for fn in ("linear", "glu"):
+        def run(v):
+            return dense.linear(v, w, activation="gelu") if fn == "linear" else dense.glu(v, w, wu)
+        xin = x.clone().requires_grad_()
+        (dx,) = torch.autograd.grad(run(xin), xin, dy)
+        d = rand(dev, n, k, dt=torch.float32, seed=56)
+        d = d / d.norm()
+        slope = float((dx.double() * d.double()).sum())
+        up, down = (float((run(x + s * h * d).double() * dy.double()).sum()) for s in (1, -1))
+        _, slack, *_ = linear64(x, w, None, None, "gelu") if fn == "linear" else glu64(x, w, wu, "silu")
+        noise = 2 * float((dy.double().abs() * (slack + 2.0 ** -24)).sum()) / (2 * h)
+        rounding = 2.0 ** -24 * float((x.abs().double() * dx.abs().double()).sum()) / h
+        along = [(d.double() @ q.double().t()).abs() for q in (w, wu)]
+        u = (x.double() @ wu.double().t()).abs() + 1
+        third = (2 * along[0] ** 3) if fn == "linear" else (2 * along[0] ** 3 * u + 3 * 1.2 * along[0] ** 2 * along[1])
+        bend = h * h / 6 * float((dy.double().abs() * third).sum()) * 2
+        assert abs((up - down) / (2 * h) - slope) <= noise + rounding + bend
+
+
+def test_repeatable_streams_and_graphs(dev):
+    from bcfft import dense
+    x, w, wu = (rand(dev, *s, dt=torch.bfloat16, seed=61 + i, scale=0.1) for i, s in enumerate(((200, 1024), (512, 1024), (512, 1024))))
+    dh = rand(dev, 200, 512, dt=torch.bfloat16, seed=65)
+
+    def step(v):
+        ins = [t.detach().clone().requires_grad_() for t in (v, w, wu)]
+        h = dense.glu(*ins)
+        return (h.detach(),) + torch.autograd.grad(h, ins, dh)
+
+    first = step(x)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, step(x)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(first, other))
+    static = x.clone()
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):                                    # two graphs: each its own workspace
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(static)
+            y = dense.linear(static, w, activation="gelu")
+        graphs.append((g, out, y))
+    for scale in (1.0, 0.5, -2.0):
+        static.copy_(x * scale)
+        for g, _, _ in graphs:
+            g.replay()
+        want, yw = step(x * scale), dense.linear(x * scale, w, activation="gelu")
+        torch.cuda.synchronize()
+        for _, out, y in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want)) and torch.equal(y, yw)
+
+
+def test_refusals(dev):
+    from bcfft import dense
+    x, w = torch.randn(3, 64, device=dev), torch.randn(32, 64, device=dev)
+    with pytest.raises(ValueError, match="weight"):
+        dense.linear(x, w[:, :32])
+    with pytest.raises(ValueError, match="w_up"):
+        dense.glu(x, w, w[:16])
+    with pytest.raises(ValueError, match="bias"):
+        dense.linear(x, w, torch.zeros(31, device=dev))
+    with pytest.raises(ValueError, match="residual"):
+        dense.linear(x, w, residual=torch.zeros(1, 32, device=dev))
+    with pytest.raises(TypeError, match="one dtype"):
+        dense.linear(x, w.half())
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        dense.linear(x.double(), w.double())
+    with pytest.raises(ValueError, match="activation"):
+        dense.linear(x, w, activation="tanh")
+    with pytest.raises(ValueError, match="weight is on cpu"):
+        dense.linear(x, w.cpu())
+    with pytest.raises(ValueError, match="scalar"):
+        dense.linear(torch.tensor(1.0, device=dev), w)
