@@ -300,14 +300,16 @@ int bcfft_distill_topk_backward(const void* logits, int dtype, int64_t n_rows, i
  *   linear: y = act(x w^T + bias) + residual          glu: h = act(x w_gate^T) * (x w_up^T)
  * x (n_tokens, in_features) with x_stride elements between rows; w, w_gate, w_up (out_features,
  * in_features) contiguous; bias (out_features) or NULL; residual (n_tokens, out_features) with r_stride, or
- * NULL; y / h (n_tokens, out_features) contiguous. Everything of one dtype, element-aligned: rows that start
- * on 16 bytes run the direct-to-LDS kernels. Products accumulate in fp32, bias, activation and residual are
+ * NULL; y / h (n_tokens, out_features) contiguous. Everything of one dtype. x, the weights and dy start on 16
+ * bytes, and so do the rows of x and dy where their features fill whole 16-byte pieces; other features are
+ * copied to padded rows in the workspace first (the forwards of up to 32 rows read them as they are). The
+ * rest is element-aligned. Products accumulate in fp32, bias, activation and residual are
  * applied there, one rounding to dtype. Features and strides up to 2^20 (the glu backward: 2 out_features), up to 2^23
  * tokens; n_tokens == 0 is a no-op.
  *   z / gu: fp32, what the backward needs: x w^T + bias (n_tokens, out_features), or g then u
  *     (2, n_tokens, out_features); NULL where there is no backward (linear: also without activation).
- * workspace: bcfft_dense_workspace_bytes(op, ...) bytes, 16-B aligned: partial sums of products whose k is
- *   split over workgroups, added in a fixed order (deterministic); the forwards run unsplit without it.
+ * workspace: bcfft_dense_workspace_bytes(op, ...) bytes, 16-B aligned (NULL if 0): padded copies, dz, and the
+ *   partial sums of products whose k is split over workgroups, added in a fixed order (deterministic).
  * GELU is the exact form, z * Phi(z). */
 enum bcfft_act { BCFFT_ACT_NONE = 0, BCFFT_ACT_RELU = 1, BCFFT_ACT_SILU = 2, BCFFT_ACT_GELU = 3 };
 enum bcfft_dense_op { BCFFT_DENSE_LINEAR = 0, BCFFT_DENSE_GLU = 1, BCFFT_DENSE_LINEAR_BACKWARD = 2,

@@ -24,11 +24,23 @@ _LINEAR, _GLU, _LINEAR_BACKWARD, _GLU_BACKWARD = range(4)
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    """(..., K) -> (N, K) with adjacent elements; rows of a stride stay where they are."""
+    """(..., K) -> (N, K) as the library takes it: adjacent elements, a 16-byte aligned start, and rows that
+    start on 16 bytes too if K fills whole 16-byte pieces. Rows of such a stride stay where they are."""
     x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x.shape[0] > 1 and not x.shape[1] <= x.stride(0) <= MAX_FEATURES or x.shape[1] > 1 and x.stride(1) != 1:
+    n, k = x.shape
+    e = x.element_size()
+    if (n > 1 and (not k <= x.stride(0) <= MAX_FEATURES or x.stride(0) * e % 16 and k * e % 16 == 0) or
+            k > 1 and x.stride(1) != 1):
         x = x.contiguous()
-    return x
+    return _aligned(x)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+
+
+def _weight(w: torch.Tensor) -> torch.Tensor:
+    return _aligned(w.detach().contiguous())
 
 
 def _stride(x: torch.Tensor) -> int:
@@ -97,7 +109,7 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        x2d, w = _rows(x.detach()), weight.detach().contiguous()
+        x2d, w = _rows(x.detach()), _weight(weight)
         b = None if bias is None else bias.detach().contiguous()
         r = None if residual is None else _rows(residual.detach())
         keep = act != 0 and any(ctx.needs_input_grad[:3])
@@ -111,7 +123,7 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        x2d, w, d2d = _rows(x.detach()), weight.detach().contiguous(), _rows(dy)
+        x2d, w, d2d = _rows(x.detach()), _weight(weight), _rows(dy)
         n, k = x2d.shape
         m = w.shape[0]
         dx = torch.empty((n, k), dtype=x.dtype, device=x.device) if need_x else None
@@ -146,7 +158,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
                                     (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act)
     b = None if bias is None else bias.detach().contiguous()
-    y, _ = _linear_forward(_rows(x.detach()), weight.detach().contiguous(), b,
+    y, _ = _linear_forward(_rows(x.detach()), _weight(weight), b,
                            None if residual is None else _rows(residual.detach()), act, False)
     return y.view(*lead, weight.shape[0])
 
@@ -171,7 +183,7 @@ class _Glu(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act):
-        x2d, wg, wu = _rows(x.detach()), w_gate.detach().contiguous(), w_up.detach().contiguous()
+        x2d, wg, wu = _rows(x.detach()), _weight(w_gate), _weight(w_up)
         h, gu = _glu_forward(x2d, wg, wu, act, True)
         ctx.save_for_backward(x, w_gate, w_up, gu)
         ctx.act = act
@@ -182,7 +194,7 @@ class _Glu(torch.autograd.Function):
     def backward(ctx, dh):
         x, w_gate, w_up, gu = ctx.saved_tensors
         need_x, need_g, need_u = ctx.needs_input_grad[:3]
-        x2d, wg, wu, d2d = _rows(x.detach()), w_gate.detach().contiguous(), w_up.detach().contiguous(), _rows(dh)
+        x2d, wg, wu, d2d = _rows(x.detach()), _weight(w_gate), _weight(w_up), _rows(dh)
         n, k = x2d.shape
         m = wg.shape[0]
         dx = torch.empty((n, k), dtype=x.dtype, device=x.device) if need_x else None
@@ -211,5 +223,5 @@ def glu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation
         raise ValueError(f"bcfft.dense.glu: out_features = {w_gate.shape[0]}, at most {MAX_FEATURES // 2}")
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         return _Glu.apply(x, w_gate, w_up, act)
-    h, _ = _glu_forward(_rows(x.detach()), w_gate.detach().contiguous(), w_up.detach().contiguous(), act, False)
+    h, _ = _glu_forward(_rows(x.detach()), _weight(w_gate), _weight(w_up), act, False)
     return h.view(*x.shape[:-1], w_gate.shape[0])

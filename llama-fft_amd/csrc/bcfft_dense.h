@@ -13,6 +13,7 @@ struct DenseArgs {
   int64_t lda, ldb;                      // elements between rows (by rows) or between k-rows (by columns)
   int64_t k;                             // elements of k per segment
   int64_t m, n;                          // output rows and columns (GLU: columns of h)
+  int64_t am, bn;                        // by columns: elements that may be read of a k-row of a, b (>= m, n)
   const void* bias;                      // (n) or null
   const void* res;                       // (m, n) with stride ldr, or null
   int64_t ldr;
@@ -26,11 +27,22 @@ struct DzArgs {
   const void* dy;
   int64_t ldd;
   const float* z;                        // pre-activation, or g and u
-  void* dz;                              // dz, or rows of dg, du
+  void* dz;                              // rows of dz, ldz elements apart; or rows of dg and, ldz / 2 further, du
+  int64_t ldz;
   float* part;                           // column sums per slice of rows, or null
   int64_t m, n;
   int act;
 };
+
+// how a product is cut: tile kind (0: few rows, 1: 128 x 128, 2: 256 x 128, 3: 256 x 256) and slices of k
+struct Shape {
+  int kind, kz;
+};
+// C = A B^T of one dtype; A and B by rows or by columns (bcfft_dense_{f32,f16,bf16}.hip)
+enum DenseLayout { DENSE_ROWS, DENSE_GLU, DENSE_ROWS_COLS, DENSE_COLS };
+void launch_product_f32(const DenseArgs& a, DenseLayout layout, Shape sh, hipStream_t s);
+void launch_product_f16(const DenseArgs& a, DenseLayout layout, Shape sh, hipStream_t s);
+void launch_product_bf16(const DenseArgs& a, DenseLayout layout, Shape sh, hipStream_t s);
 
 // 16 bytes at an address aligned to the element only (gfx950 serves unaligned global accesses)
 template <int E>

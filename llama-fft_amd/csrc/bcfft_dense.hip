@@ -5,472 +5,80 @@
 // and their gradients dz W, dz^T x, (dg Wg + du Wu), (dg, du)^T x with dz = dy act'(z), dg = dh u act'(g),
 // du = dh act(g).
 //
-// One tile kernel computes C[m][n] = sum_k A(m, k) B(n, k) for all of them. Either operand lies "by rows"
-// (k contiguous) or "by columns" (m or n contiguous): forward by rows / by rows, dx by rows / by columns,
-// dw by columns / by columns. Products of 16-bit operands are exact in the fp32 accumulators of the
-// matrix cores (v_mfma_f32_16x16x32), fp32 operands use v_mfma_f32_16x16x4; one rounding at the end.
+// The products run in bcfft_dense_{f32,f16,bf16}.hip; here are the elementwise kernels between them, the choice
+// of tiles and the C entry points.
 #include "bcfft_dense.h"
 
 #include <type_traits>
 
 namespace bcfft {
 
-// ------------------------------------------------------------------ matrix-core step
-// frag: 16 bytes of k per lane: row lane & 15, 16-byte piece lane >> 4 of 64 bytes. D's rows are a's
-// rows, four per lane; D's columns b's rows.
-template <int DT>
-__device__ __forceinline__ f32x4 mma(uint4 a, uint4 b, f32x4 c) {
-  if constexpr (DT == BCFFT_BF16) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  } else if constexpr (DT == BCFFT_F16) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  } else {
-    // lane group g holds k = 4 g .. 4 g + 3: step j multiplies k = 4 g + j of both sides
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
-  }
-}
-
-// ------------------------------------------------------------------ operand tiles
-// A tile holds R rows of 128 bytes of k (64 16-bit or 32 fp32 elements), R * 8 pieces of 16 bytes. Piece q
-// of the tile lies at LDS byte 16 q (what the direct-to-LDS loads require: lane order), and which global
-// piece it is carries the bank swizzle:
-//   by rows:    q = 8 row + c holds piece c ^ (row & 7) of the row's 128 bytes
-//   by columns: q = CPR krow + c holds piece c ^ swizzle(krow) of the k-row's R elements (CPR = R E / 16)
-template <int DT, int R, bool COL, int NT>
-struct Operand {
-  static constexpr int E = DT == BCFFT_F32 ? 4 : 2;
-  static constexpr int EPC = 16 / E;                  // elements per piece
-  static constexpr int BK = 128 / E;                  // k per tile
-  static constexpr int CPR = R * E / 16;              // pieces per k-row (by columns)
-  static constexpr int PER = R * 8 / NT;              // pieces per thread
-  static_assert(R * 8 % NT == 0 && NT % 64 == 0, "whole pieces per thread");
-
-  __device__ static __forceinline__ int swizzle(int krow) {
-    if constexpr (DT == BCFFT_F32) return ((krow >> 2 & 3) << 2) & (CPR - 1);
-    else return (((krow & 3) | (krow >> 3 & 3) << 2) << 1) & (CPR - 1);
-  }
-  // tile row (or k-row) and global piece of this thread's i-th piece
-  __device__ static __forceinline__ void place(int i, int& row, int& piece) {
-    const int q = i * NT + (int)threadIdx.x;
-    if constexpr (COL) {
-      row = q / CPR;
-      piece = (q % CPR) ^ swizzle(row);
-    } else {
-      row = q >> 3;
-      piece = (q & 7) ^ (row & 7);
-    }
-  }
-  // byte offsets from the tile's first element, rows (columns) past `dim` repeating the last valid ones:
-  // they only reach output rows that are not stored
-  __device__ static __forceinline__ void offsets(uint32_t (&off)[PER], int64_t dim, int64_t ld) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      int row, piece;
-      place(i, row, piece);
-      if constexpr (COL) {
-        const int last = (int)(dim / EPC) - 1;
-        off[i] = (uint32_t)(row * ld * E) + (uint32_t)(piece < last ? piece : last) * 16u;
-      } else {
-        const int64_t r = row < dim ? row : dim - 1;
-        off[i] = (uint32_t)(r * ld * E) + (uint32_t)piece * 16u;
-      }
-    }
-  }
-  // any address and any size: a piece that is not whole inside (dim, kleft) is put together by element,
-  // zero outside
-  __device__ static __forceinline__ uint4 fetch(const char* base, int64_t dim, int64_t ld, int64_t kleft, int i) {
-    int row, piece;
-    place(i, row, piece);
-    const int64_t r = COL ? piece * EPC : row, k = COL ? row : piece * EPC;
-    const int64_t along = COL ? dim - r : kleft - k, across = COL ? kleft - k : dim - r;
-    const char* p = base + (COL ? k * ld + r : r * ld + k) * E;
-    if (across <= 0 || along <= 0) return make_uint4(0, 0, 0, 0);
-    if (along >= EPC) {
-      const Unaligned16<E> u = *reinterpret_cast<const Unaligned16<E>*>(p);
-      return make_uint4(u.w[0], u.w[1], u.w[2], u.w[3]);
-    }
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < EPC - 1; ++j) {
-      if (j < along) {
-        if constexpr (E == 4) w[j] = ((const uint32_t*)p)[j];
-        else w[j / 2] |= (uint32_t)((const uint16_t*)p)[j] << 16 * (j & 1);
-      }
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-
-// Fragment reads: rows base .. base + 15 of a tile for the kk-th 64 bytes of k
-template <int DT, int R, bool COL>
-struct Fragments {
-  static constexpr int E = DT == BCFFT_F32 ? 4 : 2;
-  static constexpr int CPR = R * E / 16;
-  static constexpr int RB = R * E;
-  int lane_off, key;                                   // by columns: the row part, and the swizzle
-
-  __device__ __forceinline__ void init(int lane) {
-    const int g = lane >> 4, l = lane & 15;
-    if constexpr (!COL) {
-      lane_off = l * 128 + ((g ^ (l & 7)) << 4);
-      key = 0;
-    } else if constexpr (DT == BCFFT_F32) {
-      lane_off = 4 * g * RB + (l & 3) * 4;
-      key = ((g << 2) & (CPR - 1)) ^ (l >> 2);
-    } else {
-      const int q4 = l >> 2, p4 = l & 3;
-      lane_off = (8 * g + q4) * RB + (p4 & 1) * 8;
-      key = (((q4 | g << 2) << 1) & (CPR - 1)) ^ (p4 >> 1);
-    }
-  }
-  __device__ __forceinline__ uint4 read(const char* tile, int base, int kk) const {
-    if constexpr (!COL) {
-      return *reinterpret_cast<const uint4*>(tile + base * 128 + (lane_off ^ (kk << 6)));
-    } else if constexpr (DT == BCFFT_F32) {
-      const char* p = tile + lane_off + (((base / 4) ^ key) << 4) + 16 * kk * RB;
-      return make_uint4(*(const uint32_t*)p, *(const uint32_t*)(p + RB), *(const uint32_t*)(p + 2 * RB),
-                        *(const uint32_t*)(p + 3 * RB));
-    } else {
-      // a 16-lane group's transposed read: rows 4 of k, each lane receives one column's four values
-      const char* p = tile + lane_off + (((base / 8) ^ key) << 4) + 32 * kk * RB;
-      using V = __attribute__((address_space(3))) s16x4*;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((V)(p));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((V)(p + 4 * RB));
-      const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
-      return make_uint4(a.x, a.y, b.x, b.y);
-    }
-  }
-};
-
-// LDS[lds + 16 lane] <- 16 bytes at base + off (per lane). The compiler does not count these loads: the
-// loop's own wait and barrier order them.
-__device__ __forceinline__ void dma16_base(const char* base, uint32_t off, uint32_t lds) {
-  uint32_t keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(off), "s"(base), "s"(lds) : "memory");
-}
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-// every load into LDS and every LDS access of this wave complete, then the workgroup's rendezvous
-__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
-// ------------------------------------------------------------------ the tile kernel
-// WM x WN waves, each (BM / WM) x (BN / WN) of the BM x BN tile in accumulators; two LDS buffers, the next
-// tile on its way while the current one is multiplied, one barrier per tile.
-// GLU: B's tile is BN / 2 rows of the gate weight and BN / 2 of the up weight, and a wave holds the same
-// columns of both, so the product of the two needs no exchange.
-// ASYNC: operands whose rows start 16-byte aligned go to LDS directly; else through registers.
-template <int DT, bool CA, bool CB, int BM, int BN, int WM, int WN, bool ASYNC, bool GLU>
-__global__ __launch_bounds__(64 * WM * WN, 1) void bc_dense_tile_kernel(DenseArgs a) {
-  constexpr int NT = 64 * WM * WN, E = DT == BCFFT_F32 ? 4 : 2, BK = 128 / E;
-  constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  constexpr int NB = GLU ? 2 : 1, BR = BN / NB;        // B's sources and rows of each
-  constexpr int ABYTES = BM * 128, BBYTES = BN * 128, BUF = ABYTES + BBYTES;
-  using OA = Operand<DT, BM, CA, NT>;
-  using OB = Operand<DT, BR, CB, NT>;
-  static_assert(!GLU || !CB, "the gated form reads weights by rows");
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = wave / WN, wn = wave % WN;
-
-  // workgroups of one XCD (round-robin by id) take a contiguous run of tiles; within it, columns of GROUP
-  // row tiles, so that the operands of the tiles in flight fit the XCD's L2
-  const int mt = (int)((a.m + BM - 1) / BM), nt = (int)((a.n + BR - 1) / BR);
-  const int total = mt * nt;
-  int id = blockIdx.x;
-  {
-    const int per = total / 8, extra = total % 8, xcd = id % 8, slot = id / 8;
-    id = xcd * per + (xcd < extra ? xcd : extra) + slot;
-  }
-  constexpr int GROUP = 8;
-  const int band = id / (GROUP * nt), first = band * GROUP;
-  const int high = mt - first < GROUP ? mt - first : GROUP;
-  const int tm = first + (id - band * GROUP * nt) % high, tn = (id - band * GROUP * nt) / high;
-  const int64_t m0 = (int64_t)uniform(tm) * BM, n0 = (int64_t)uniform(tn) * BR;
-  const int64_t mleft = a.m - m0, nleft = a.n - n0;
-
-  // this slice's run of k tiles
-  const int tps = (int)((a.k + BK - 1) / BK);          // tiles per segment
-  const int tiles = tps * a.segs;
-  const int t0 = uniform((int)((int64_t)tiles * blockIdx.y / a.kz));
-  const int t1 = uniform((int)((int64_t)tiles * (blockIdx.y + 1) / a.kz));
-
-  uint32_t offa[OA::PER], offb[OB::PER];
-  if constexpr (ASYNC) {
-    OA::offsets(offa, mleft, a.lda);
-    OB::offsets(offb, nleft, a.ldb);
-  }
-  auto base_a = [&](int seg, int64_t k) {
-    return (const char*)(seg ? a.a[1] : a.a[0]) + (CA ? k * a.lda + m0 : m0 * a.lda + k) * E;
-  };
-  auto base_b = [&](int src, int64_t k) {
-    return (const char*)(src ? a.b[1] : a.b[0]) + (CB ? k * a.ldb + n0 : n0 * a.ldb + k) * E;
-  };
-  uint4 ra[ASYNC ? 1 : OA::PER], rb[ASYNC ? 1 : NB * OB::PER];
-  const uint32_t lds0 = lds_addr(lds);
-  const uint32_t wave_lds = (uint32_t)__builtin_amdgcn_readfirstlane(wave) * 1024u;
-  int seg = uniform(t0 / tps);                         // where the next tile of k lies
-  int64_t at = (int64_t)(t0 - seg * tps) * BK;
-  // the next tile on its way into buffer `buf`
-  auto stage = [&](int buf) {
-    const int64_t k = at;
-    const int sg = seg;
-    at += BK;
-    if (at >= a.k) at = 0, ++seg;
-    if constexpr (ASYNC) {
-      if (k + BK <= a.k) {
-        const uint32_t l = lds0 + buf * BUF + wave_lds;
-        const char* pa = base_a(sg, k);
-#pragma unroll
-        for (int i = 0; i < OA::PER; ++i) dma16_base(pa, offa[i], l + i * NT * 16);
-#pragma unroll
-        for (int s = 0; s < NB; ++s) {
-          const char* pb = base_b(GLU ? s : sg, k);
-#pragma unroll
-          for (int i = 0; i < OB::PER; ++i) dma16_base(pb, offb[i], l + ABYTES + s * BR * 128 + i * NT * 16);
-        }
-        return;
-      }
-    }
-    // the last, partial tile of k, or operands that are not 16-byte aligned
-    char* out = lds + buf * BUF + tid * 16;
-#pragma unroll
-    for (int i = 0; i < OA::PER; ++i) {
-      const uint4 v = OA::fetch(base_a(sg, k), mleft, a.lda, a.k - k, i);
-      if constexpr (ASYNC) *reinterpret_cast<uint4*>(out + i * NT * 16) = v;
-      else ra[i] = v;
-    }
-#pragma unroll
-    for (int s = 0; s < NB; ++s) {
-#pragma unroll
-      for (int i = 0; i < OB::PER; ++i) {
-        const uint4 v = OB::fetch(base_b(GLU ? s : sg, k), nleft, a.ldb, a.k - k, i);
-        if constexpr (ASYNC) *reinterpret_cast<uint4*>(out + ABYTES + s * BR * 128 + i * NT * 16) = v;
-        else rb[s * OB::PER + i] = v;
-      }
-    }
-  };
-  auto commit = [&](int buf) {                         // registers -> LDS (not ASYNC)
-    char* out = lds + buf * BUF + tid * 16;
-    if constexpr (!ASYNC) {
-#pragma unroll
-      for (int i = 0; i < OA::PER; ++i) *reinterpret_cast<uint4*>(out + i * NT * 16) = ra[i];
-#pragma unroll
-      for (int s = 0; s < NB; ++s)
-#pragma unroll
-        for (int i = 0; i < OB::PER; ++i)
-          *reinterpret_cast<uint4*>(out + ABYTES + s * BR * 128 + i * NT * 16) = rb[s * OB::PER + i];
-    }
-  };
-
-  Fragments<DT, BM, CA> fa;
-  Fragments<DT, BR, CB> fb;
-  fa.init(lane);
-  fb.init(lane);
-  f32x4 acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  if (t0 < t1) {
-    stage(0);
-    commit(0);
-  }
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    tile_barrier();
-    if (t + 1 < t1) stage(buf ^ 1);
-    const char* ta = lds + buf * BUF;
-    const char* tb = ta + ABYTES;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      uint4 vb[FN];
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        if constexpr (GLU)
-          vb[j] = fb.read(tb + (j < FN / 2 ? 0 : BR * 128), wn * (TN / 2) + (j % (FN / 2)) * 16, kk);
-        else
-          vb[j] = fb.read(tb, wn * TN + j * 16, kk);
-      }
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const uint4 va = fa.read(ta, wm * TM + i * 16, kk);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mma<DT>(vb[j], va, acc[i][j]);
-      }
-    }
-    if (t + 1 < t1) commit(buf ^ 1);
-  }
-
-  // lane: row m0 + .. + (lane & 15), four consecutive columns from 4 (lane >> 4)
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int64_t m = m0 + wm * TM + i * 16 + (lane & 15);
-    if (m >= a.m) continue;
-#pragma unroll
-    for (int j = 0; j < FN / NB; ++j) {
-      const int64_t n = n0 + wn * (TN / NB) + j * 16 + 4 * (lane >> 4);
-      if (n >= a.n) continue;
-      const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
-      if constexpr (GLU) {
-        if (a.kz > 1) {
-          store_partial(a, blockIdx.y, m, n, acc[i][j], cnt);
-          store_partial(a, blockIdx.y, m, a.n + n, acc[i][j + FN / 2], cnt);
-        } else {
-          finish_glu<DT>(a, m, n, acc[i][j], acc[i][j + FN / 2], cnt);
-        }
-      } else {
-        if (a.kz > 1) store_partial(a, blockIdx.y, m, n, acc[i][j], cnt);
-        else finish_linear<DT>(a, m, n, acc[i][j], cnt);
-      }
-    }
-  }
-}
-
-// sums the slices of a split k in order and finishes the output
-template <int DT, bool GLU>
-__global__ __launch_bounds__(256) void bc_dense_finish_kernel(DenseArgs a) {
-  const int64_t quads = (a.n + 3) / 4, total = quads * a.m;
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
-    const int64_t m = q / quads, n = (q - m * quads) * 4;
-    const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
-    f32x4 g = load_partials(a, m, n, cnt);
-    if constexpr (GLU) finish_glu<DT>(a, m, n, g, load_partials(a, m, a.n + n, cnt), cnt);
-    else finish_linear<DT>(a, m, n, g, cnt);
-  }
-}
-
-// ------------------------------------------------------------------ few rows
-// Up to 16 MT rows of x (decode): bound by the weights' single read. A workgroup takes 16 rows of W (and 16
-// of the other weight, GLU), its KW waves a part of k each, straight from memory into the fragments; x comes
-// out of L2. The waves' sums meet in LDS.
-template <int DT, int MT, int KW, bool GLU>
-__global__ __launch_bounds__(64 * KW) void bc_dense_rows_kernel(DenseArgs a) {
-  constexpr int E = DT == BCFFT_F32 ? 4 : 2, EPC = 16 / E, BK = 128 / E, NB = GLU ? 2 : 1;
-  constexpr int UNROLL = 4;
-  __shared__ f32x4 part[KW][NB * MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l = lane & 15;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int64_t wrow = n0 + l < a.n ? n0 + l : a.n - 1;       // repeated rows are not stored
-  const char* pw[NB];
-#pragma unroll
-  for (int s = 0; s < NB; ++s) pw[s] = (const char*)a.b[s] + wrow * a.ldb * E;
-  const char* px[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) px[i] = (const char*)a.a[0] + (16 * i + l < a.m ? 16 * i + l : a.m - 1) * a.lda * E;
-  const int64_t tiles = (a.k + BK - 1) / BK;
-  const int64_t t0 = tiles * wave / KW, t1 = tiles * (wave + 1) / KW;
-
-  f32x4 acc[NB][MT];
-#pragma unroll
-  for (int s = 0; s < NB; ++s)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) acc[s][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto load = [&](const char* p, int64_t k) {          // 16 bytes of k, whatever the address
-    const Unaligned16<E> u = *reinterpret_cast<const Unaligned16<E>*>(p + k * E);
-    return make_uint4(u.w[0], u.w[1], u.w[2], u.w[3]);
-  };
-  auto step = [&](const uint4 (&w)[NB], const uint4 (&x)[MT]) {
-#pragma unroll
-    for (int s = 0; s < NB; ++s)
-#pragma unroll
-      for (int i = 0; i < MT; ++i) acc[s][i] = mma<DT>(w[s], x[i], acc[s][i]);
-  };
-  int64_t t = t0;
-  for (; t + UNROLL <= t1 && (t + UNROLL) * BK <= a.k; t += UNROLL) {
-    uint4 w[UNROLL][2][NB], x[UNROLL][2][MT];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int64_t k = (t + u) * BK + (g + 4 * kk) * EPC;
-#pragma unroll
-        for (int s = 0; s < NB; ++s) w[u][kk][s] = load(pw[s], k);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) x[u][kk][i] = load(px[i], k);
-      }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) step(w[u][kk], x[u][kk]);
-  }
-  for (; t < t1; ++t) {
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const int64_t k = t * BK + (g + 4 * kk) * EPC;
-      uint4 w[NB], x[MT];
-#pragma unroll
-      for (int s = 0; s < NB; ++s) w[s] = load_part<E>(pw[s], k, a.k);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) x[i] = load_part<E>(px[i], k, a.k);
-      step(w, x);
-    }
-  }
-#pragma unroll
-  for (int s = 0; s < NB; ++s)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) part[wave][s * MT + i][lane] = acc[s][i];
-  __syncthreads();
-  for (int i = wave; i < MT; i += KW) {
-    const int64_t m = 16 * i + l, n = n0 + 4 * g;
-    if (m >= a.m || n >= a.n) continue;
-    f32x4 v[NB];
-#pragma unroll
-    for (int s = 0; s < NB; ++s) {
-      v[s] = part[0][s * MT + i][lane];
-#pragma unroll
-      for (int w = 1; w < KW; ++w) v[s] += part[w][s * MT + i][lane];
-    }
-    const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
-    if constexpr (GLU) finish_glu<DT>(a, m, n, v[0], v[NB - 1], cnt);
-    else finish_linear<DT>(a, m, n, v[0], cnt);
-  }
-}
-
 // ------------------------------------------------------------------ elementwise part of the backward
 // dz = dy act'(z) as the next products' operand, rounded once to dtype, and each column's sum over 64 rows
 // of the unrounded dz (fp32) for the bias gradient. Thread: 4 columns; workgroup: 1024 columns x 64 rows.
+// Both are bound by memory: 4 rows of 64 column quads per pass, the row lanes' sums joined in LDS.
 constexpr int DZ_ROWS = 64;
 template <int DT>
 __global__ __launch_bounds__(256) void bc_dense_dz_kernel(DzArgs a) {
-  const int64_t n = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
-  if (n >= a.n) return;
+  __shared__ float sums[4][64][5];
+  const int quad = threadIdx.x & 63, lane = threadIdx.x >> 6;
+  const int64_t n = ((int64_t)blockIdx.y * 64 + quad) * 4;
+  const int64_t m0 = (int64_t)blockIdx.x * DZ_ROWS;
   const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
-  const int64_t m0 = (int64_t)blockIdx.x * DZ_ROWS, m1 = m0 + DZ_ROWS < a.m ? m0 + DZ_ROWS : a.m;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t m = m0; m < m1; ++m) {
-    float d[4], z[4];
-    load4_at<DT>(a.dy, m * a.ldd + n, cnt, d);
-    if (a.z) {
-      load4_at<BCFFT_F32>(a.z, m * a.n + n, cnt, z);
+  if (n < a.n) {
+#pragma unroll 4
+    for (int r = 0; r < DZ_ROWS / 4; ++r) {
+      const int64_t m = m0 + 4 * r + lane;
+      if (m >= a.m) break;
+      float d[4], z[4];
+      load4_at<DT>(a.dy, m * a.ldd + n, cnt, d);
+      if (a.z) {
+        load4_at<BCFFT_F32>(a.z, m * a.n + n, cnt, z);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float s, v;
-        act_both(a.act, z[j], v, s);
-        d[j] *= s;
+        for (int j = 0; j < 4; ++j) {
+          float s, v;
+          act_both(a.act, z[j], v, s);
+          d[j] *= s;
+        }
       }
-    }
-    if (a.dz) store4_at<DT>(a.dz, m * a.n + n, cnt, d);
+      if (a.dz) store4_at<DT>(a.dz, m * a.ldz + n, cnt, d);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] += d[j];
+      for (int j = 0; j < 4; ++j) sum[j] += d[j];
+    }
   }
-  if (a.part)
-    for (int j = 0; j < cnt; ++j) a.part[(int64_t)blockIdx.x * a.n + n + j] = sum[j];
+  if (!a.part) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sums[lane][quad][j] = sum[j];
+  __syncthreads();
+  const int64_t col = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  if (col < a.n) {
+    const int q = threadIdx.x >> 2, j = threadIdx.x & 3;
+    a.part[(int64_t)blockIdx.x * a.n + col] = (sums[0][q][j] + sums[1][q][j]) + (sums[2][q][j] + sums[3][q][j]);
+  }
 }
+// 32 columns, 8 lanes of slices each
 template <int DT>
 __global__ __launch_bounds__(256) void bc_dense_db_kernel(const float* __restrict__ part, int64_t slices, int64_t n,
                                                           void* __restrict__ db) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
+  __shared__ double sums[8][32];
+  const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + c;
   double s = 0.0;
-  for (int64_t k = 0; k < slices; ++k) s += part[k * n + i];
-  const float v[4] = {(float)s, 0.f, 0.f, 0.f};
-  store4_at<DT>(db, i, 1, v);
+  if (i < n) {
+#pragma unroll 4
+    for (int64_t k = lane; k < slices; k += 8) s += part[k * n + i];
+  }
+  sums[lane][c] = s;
+  __syncthreads();
+  if (lane == 0 && i < n) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sums[k][c];
+    const float v[4] = {(float)s, 0.f, 0.f, 0.f};
+    store4_at<DT>(db, i, 1, v);
+  }
 }
-// dg = dh u act'(g) and du = dh act(g), side by side in rows of 2 n
+// dg = dh u act'(g) and du = dh act(g), side by side in a row
 template <int DT>
 __global__ __launch_bounds__(256) void bc_dense_dgu_kernel(DzArgs a) {
   const int64_t quads = (a.n + 3) / 4, total = quads * a.m;
@@ -488,79 +96,45 @@ __global__ __launch_bounds__(256) void bc_dense_dgu_kernel(DzArgs a) {
       dg[j] = d[j] * u[j] * s;
       du[j] = d[j] * v;
     }
-    store4_at<DT>(a.dz, m * 2 * a.n + n, cnt, dg);
-    store4_at<DT>(a.dz, m * 2 * a.n + a.n + n, cnt, du);
+    store4_at<DT>(a.dz, m * a.ldz + n, cnt, dg);
+    store4_at<DT>(a.dz, m * a.ldz + a.ldz / 2 + n, cnt, du);
+  }
+}
+
+// rows of `cols` elements, 16-byte aligned and padded with zeros to whole 16-byte pieces: operands whose rows
+// do not start on 16 bytes run the same direct-to-LDS kernels (one copy of the operand at memory speed,
+// against products at a third of the rate with loads through registers)
+template <int E>
+__global__ __launch_bounds__(256) void bc_dense_pack_kernel(const char* __restrict__ src, int64_t ld, int64_t rows,
+                                                            int64_t cols, char* __restrict__ dst) {
+  constexpr int EPC = 16 / E;
+  const int64_t pieces = (cols + EPC - 1) / EPC, total = pieces * rows;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
+    const int64_t r = q / pieces, c = q - r * pieces;
+    *reinterpret_cast<uint4*>(dst + q * 16) = load_part<E>(src + r * ld * E, c * EPC, cols);
   }
 }
 
 // ------------------------------------------------------------------ launches
-struct Shape {                                         // how a product is cut: tile kind, slices of k
-  int kind, kz;                                        // kind 0: few rows; 1: 128 x 128; 2: 256 x 128; 3: 256 x 256
-};
-
-static bool aligned_operand(const void* p, int64_t ld, int64_t dim, bool col, int e) {
-  return ((uintptr_t)p & 15) == 0 && ld * e % 16 == 0 && (!col || dim * e % 16 == 0);
-}
-
-template <int DT, bool CA, bool CB, int BM, int BN, int WM, int WN, bool ASYNC, bool GLU>
-static void launch_tile(const DenseArgs& a, hipStream_t s) {
-  constexpr int BR = GLU ? BN / 2 : BN;
-  constexpr unsigned lds = 2 * (BM + BN) * 128;
-  auto kern = bc_dense_tile_kernel<DT, CA, CB, BM, BN, WM, WN, ASYNC, GLU>;
-  if constexpr (lds > 65536) (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  const unsigned tiles = (unsigned)(((a.m + BM - 1) / BM) * ((a.n + BR - 1) / BR));
-  hipLaunchKernelGGL(kern, dim3(tiles, (unsigned)a.kz), dim3(64 * WM * WN), lds, s, a);
-}
-
-template <int DT, bool CA, bool CB, bool GLU>
-static void launch_product_as(const DenseArgs& a, Shape sh, hipStream_t s) {
-  constexpr int E = DT == BCFFT_F32 ? 4 : 2;
-  bool async = true;
-  for (int i = 0; i < a.segs; ++i) async = async && aligned_operand(a.a[i], a.lda, a.m, CA, E);
-  for (int i = 0; i < (GLU ? 2 : a.segs); ++i) async = async && aligned_operand(a.b[i], a.ldb, a.n, CB, E);
-  if (!async) launch_tile<DT, CA, CB, 128, 128, 2, 2, false, GLU>(a, s);
-  else if (sh.kind == 1) launch_tile<DT, CA, CB, 128, 128, 2, 2, true, GLU>(a, s);
-  else if (sh.kind == 2) launch_tile<DT, CA, CB, 256, 128, 4, 2, true, GLU>(a, s);
-  else launch_tile<DT, CA, CB, 256, 256, 2, 4, true, GLU>(a, s);
-  if (a.kz > 1) {
-    const int64_t quads = (a.n + 3) / 4 * a.m;
-    const unsigned blocks = (unsigned)((quads + 255) / 256 < 16384 ? (quads + 255) / 256 : 16384);
-    hipLaunchKernelGGL((bc_dense_finish_kernel<DT, GLU>), dim3(blocks), dim3(256), 0, s, a);
-  }
-}
-
-template <int DT, bool GLU>
-static void launch_rows(const DenseArgs& a, hipStream_t s) {
-  const unsigned groups = (unsigned)((a.n + 15) / 16);
-  auto go = [&](auto mt, auto kw) {
-    hipLaunchKernelGGL((bc_dense_rows_kernel<DT, mt.value, kw.value, GLU>), dim3(groups), dim3(64 * kw.value), 0, s, a);
-  };
-  using std::integral_constant;
-  if (a.m <= 16 && groups <= 512) go(integral_constant<int, 1>(), integral_constant<int, 8>());
-  else if (a.m <= 16) go(integral_constant<int, 1>(), integral_constant<int, 4>());
-  else if (groups <= 512) go(integral_constant<int, 2>(), integral_constant<int, 8>());
-  else go(integral_constant<int, 2>(), integral_constant<int, 4>());
-}
-
-// Tile and slices for an m x n product over k of `parts` column blocks per output (2: gated): the cheapest by
-// an estimate in units of one 128 x 128 x 128-byte step: workgroup rounds over the CUs times steps, and for
-// slices the partial sums' way through memory.
-static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, bool forward) {
+// Tile and slices for an m x n product over ksteps tiles of k, with `parts` products per output (2: gated):
+// the least estimated time in microseconds. step: one tile of k of one workgroup with its CU's share (16-bit:
+// measured at 8192 x 4096 x 4096; fp32: the fp32 matrix rate). Slices pay their partial sums' way through
+// memory and the finishing launch.
+static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, bool forward) {
   if (forward && m <= 32) return {0, 1};
   const int64_t cus = device_cu_count();
+  struct Kind { int kind, bm, bn, slots; double step, step32, fixed; };
+  const Kind kinds[3] = {{1, 128, 128, 2, 0.48, 1.9, 3.0}, {2, 256, 128, 1, 0.80, 3.8, 5.0}, {3, 256, 256, 1, 1.55, 7.6, 8.0}};
   Shape best{1, 1};
   double least = 1e300;
-  struct Kind { int kind, bm, bn, slots; double step; };
-  const Kind kinds[3] = {{1, 128, 128, 2, 1.15}, {2, 256, 128, 1, 1.9}, {3, 256, 256, 1, 3.4}};
   for (const Kind& q : kinds) {
-    const int64_t tiles = ((m + q.bm - 1) / q.bm) * ((n + q.bn / parts - 1) / (q.bn / parts));
-    for (int64_t kz = 1; kz <= 16 && (kz == 1 || ksteps / kz >= 8); kz *= 2) {
+    const int64_t tiles = ((m + q.bm - 1) / q.bm) * ((n * parts + q.bn - 1) / q.bn);
+    for (int64_t kz = 1; kz <= 16 && (kz == 1 || ksteps / kz >= 4); ++kz) {
       const int64_t groups = tiles * kz;
-      // groups per CU, and the share of the CU's rate they reach when fewer than `slots` run there
-      const int64_t rounds = (groups + cus * q.slots - 1) / (cus * q.slots);
-      const double per = groups >= cus * q.slots ? (double)rounds * q.slots : (double)((groups + cus - 1) / cus);
-      double cost = per * ((double)(ksteps + kz - 1) / kz + 3.0) * q.step;
-      if (kz > 1) cost += 12.0 + (double)(kz + 1) * m * n * parts * 4.0 / 2.2e6;
+      const int64_t per_cu = (groups + cus - 1) / cus;                   // the fullest CU's workgroups
+      const double step = dt == BCFFT_F32 ? q.step32 : q.step * (q.slots == 2 && per_cu == 1 ? 1.3 : 1.0);
+      double cost = (double)per_cu * ((double)((ksteps + kz - 1) / kz) * step + q.fixed);
+      if (kz > 1) cost += 4.0 + (double)(2 * kz) * m * n * parts * 4.0 / 4e6;
       if (cost < least) {
         least = cost;
         best = {q.kind, (int)kz};
@@ -570,19 +144,10 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, bool forwar
   return best;
 }
 
-template <bool CA, bool CB, bool GLU>
-static void launch_product(int dt, const DenseArgs& a, Shape sh, hipStream_t s) {
-  if constexpr (!CA && !CB) {
-    if (sh.kind == 0) {
-      if (dt == BCFFT_F32) launch_rows<BCFFT_F32, GLU>(a, s);
-      else if (dt == BCFFT_F16) launch_rows<BCFFT_F16, GLU>(a, s);
-      else launch_rows<BCFFT_BF16, GLU>(a, s);
-      return;
-    }
-  }
-  if (dt == BCFFT_F32) launch_product_as<BCFFT_F32, CA, CB, GLU>(a, sh, s);
-  else if (dt == BCFFT_F16) launch_product_as<BCFFT_F16, CA, CB, GLU>(a, sh, s);
-  else launch_product_as<BCFFT_BF16, CA, CB, GLU>(a, sh, s);
+static void launch_product(int dt, const DenseArgs& a, DenseLayout layout, Shape sh, hipStream_t s) {
+  if (dt == BCFFT_F32) launch_product_f32(a, layout, sh, s);
+  else if (dt == BCFFT_F16) launch_product_f16(a, layout, sh, s);
+  else launch_product_bf16(a, layout, sh, s);
 }
 
 static bool valid_dt(int d) { return d == BCFFT_F32 || d == BCFFT_F16 || d == BCFFT_BF16; }
@@ -594,22 +159,54 @@ static bool aligned_to(const void* p, int bytes) { return ((uintptr_t)p & (uintp
 static bool valid_sizes(int64_t n, int64_t k, int64_t m) {
   return n >= 0 && n <= (1 << 23) && k >= 1 && k <= (1 << 20) && m >= 1 && m <= (1 << 20);
 }
+static bool valid_stride(int64_t stride, int64_t features) { return stride >= features && stride <= (1 << 20); }
+// rows start on 16 bytes, or are packed because their features are no whole number of 16-byte pieces
+static bool aligned_stride(int64_t stride, int64_t rows, int64_t features, int dt) {
+  return rows <= 1 || stride * elem(dt) % 16 == 0 || features * elem(dt) % 16 != 0;
+}
 static int64_t partial_bytes(int64_t m, int64_t n, Shape sh) { return sh.kz > 1 ? round16((int64_t)sh.kz * m * n * 4) : 0; }
+// elements of a row padded to whole 16-byte pieces
+static int64_t padded(int64_t cols, int dt) { return round16(cols * elem(dt)) / elem(dt); }
+static bool whole(int64_t cols, int dt) { return cols * elem(dt) % 16 == 0; }
+static int64_t packed_bytes(int64_t rows, int64_t cols, int dt) { return rows * round16(cols * elem(dt)); }
+static const void* pack(int dt, const void* src, int64_t ld, int64_t rows, int64_t cols, char*& ws, hipStream_t s) {
+  const int64_t total = rows * padded(cols, dt) * elem(dt) / 16;
+  const unsigned blocks = (unsigned)((total + 255) / 256 < 16384 ? (total + 255) / 256 : 16384);
+  if (elem(dt) == 4) hipLaunchKernelGGL(bc_dense_pack_kernel<4>, dim3(blocks), dim3(256), 0, s, (const char*)src, ld, rows, cols, ws);
+  else hipLaunchKernelGGL(bc_dense_pack_kernel<2>, dim3(blocks), dim3(256), 0, s, (const char*)src, ld, rows, cols, ws);
+  const void* at = ws;
+  ws += packed_bytes(rows, cols, dt);
+  return at;
+}
 
-struct BackwardPlan {                                  // workspace of a backward call
+struct ForwardPlan {
+  Shape shape;
+  bool packed;                                         // x and the weights are copied to 16-byte rows
+  int64_t pack_bytes, total;
+};
+static ForwardPlan forward_plan(int64_t n, int64_t k, int64_t m, int dt, int parts) {
+  ForwardPlan p;
+  p.shape = choose(n, m, ksteps(k, dt), parts, dt, true);
+  p.packed = p.shape.kind != 0 && !whole(k, dt);       // the few-rows kernel reads any address
+  p.pack_bytes = p.packed ? packed_bytes(n + parts * m, k, dt) : 0;
+  p.total = p.pack_bytes + partial_bytes(n, parts * m, p.shape);
+  return p;
+}
+struct BackwardPlan {                                  // workspace of a backward call, in this order
   Shape dx, dw;
-  int64_t dz_bytes, part_bytes, slices, ws_dx, ws_dw, total;
+  int64_t dz_bytes, part_bytes, slices, pack_bytes, total;
 };
 static BackwardPlan backward_plan(int64_t n, int64_t k, int64_t m, int dt, int parts, int act) {
   BackwardPlan p;
-  p.dx = choose(n, k, parts * ksteps(m, dt), 1, false);
-  p.dw = choose(parts * m, k, ksteps(n, dt), 1, false);
-  p.dz_bytes = parts == 2 || act != BCFFT_ACT_NONE ? round16(n * parts * m * elem(dt)) : 0;
+  const bool split = parts == 2 && !whole(m, dt);      // dg and du are not adjacent columns
+  p.dx = choose(n, k, parts * ksteps(m, dt), 1, dt, false);
+  p.dw = choose(split ? m : parts * m, k, ksteps(n, dt), 1, dt, false);
+  p.dz_bytes = parts == 2 || act != BCFFT_ACT_NONE || !whole(m, dt) ? parts * packed_bytes(n, m, dt) : 0;
   p.slices = (n + DZ_ROWS - 1) / DZ_ROWS;
   p.part_bytes = parts == 1 ? round16(p.slices * m * 4) : 0;
-  p.ws_dx = partial_bytes(n, k, p.dx);
-  p.ws_dw = partial_bytes(parts * m, k, p.dw);
-  p.total = p.dz_bytes + p.part_bytes + (p.ws_dx > p.ws_dw ? p.ws_dx : p.ws_dw);
+  p.pack_bytes = whole(k, dt) ? 0 : packed_bytes(n + parts * m, k, dt);
+  const int64_t sx = partial_bytes(n, k, p.dx), sw = partial_bytes(split ? m : parts * m, k, p.dw);
+  p.total = p.dz_bytes + p.part_bytes + p.pack_bytes + (sx > sw ? sx : sw);
   return p;
 }
 
@@ -620,28 +217,50 @@ static void by_dtype(int dt, F&& f) {
   else f(std::integral_constant<int, BCFFT_BF16>());
 }
 
-// dx = [dz] W (parts 1) or dg Wg + du Wu (parts 2: dz holds both, rows of 2 m)
-static void launch_dx(int dt, const void* dz, int64_t ldz, const void* w0, const void* w1, int64_t n, int64_t k, int64_t m,
-                      Shape sh, void* dx, float* ws, hipStream_t s) {
+// The forwards share their operands' preparation; what differs is set by the caller
+static int run_forward(int dt, DenseArgs a, const void* w1, const ForwardPlan& p, void* workspace, int64_t bytes,
+                       hipStream_t s) {
+  if (p.total > 0 && (!workspace || bytes < p.total)) return BCFFT_ERR_ARG;
+  char* ws = (char*)workspace;
+  a.b[1] = w1;
+  a.segs = 1;
+  a.am = a.m;
+  a.bn = a.n;
+  if (p.packed) {
+    a.a[0] = pack(dt, a.a[0], a.lda, a.m, a.k, ws, s);
+    a.b[0] = pack(dt, a.b[0], a.ldb, a.n, a.k, ws, s);
+    if (w1) a.b[1] = pack(dt, w1, a.ldb, a.n, a.k, ws, s);
+    a.k = a.lda = a.ldb = padded(a.k, dt);             // the padding is zero
+  }
+  a.ws = (float*)ws;
+  a.kz = p.shape.kz;
+  launch_product(dt, a, w1 ? DENSE_GLU : DENSE_ROWS, p.shape, s);
+  return record_launch_status();
+}
+
+// dx = dz W, or dg Wg + du Wu with du `apart` elements behind dg; W's rows of kp elements
+static void launch_dx(int dt, const void* dz, int64_t ldz, int64_t apart, const void* w0, const void* w1, int64_t n,
+                      int64_t k, int64_t kp, int64_t m, Shape sh, void* dx, float* ws, hipStream_t s) {
   DenseArgs a{};
   a.a[0] = dz;
-  a.a[1] = (const char*)dz + m * elem(dt);
+  a.a[1] = (const char*)dz + apart * elem(dt);
   a.b[0] = w0;
   a.b[1] = w1;
   a.lda = ldz;
-  a.ldb = k;
+  a.ldb = kp;
   a.k = m;
   a.segs = w1 ? 2 : 1;
-  a.m = n;
+  a.m = a.am = n;
   a.n = k;
+  a.bn = kp;
   a.y = dx;
   a.ws = ws;
   a.kz = sh.kz;
-  launch_product<false, true, false>(dt, a, sh, s);
+  launch_product(dt, a, DENSE_ROWS_COLS, sh, s);
 }
-// dw[m][k] = sum over tokens of dz[token][m] x[token][k]
-static void launch_dw(int dt, const void* dz, int64_t ldz, const void* x, int64_t ldx, int64_t n, int64_t k, int64_t m,
-                      Shape sh, void* dw, float* ws, hipStream_t s) {
+// dw[m][k] = sum over tokens of dz[token][m] x[token][k]; mp, kp: readable elements of their rows
+static void launch_dw(int dt, const void* dz, int64_t ldz, int64_t mp, const void* x, int64_t ldx, int64_t kp, int64_t n,
+                      int64_t k, int64_t m, Shape sh, void* dw, float* ws, hipStream_t s) {
   DenseArgs a{};
   a.a[0] = dz;
   a.b[0] = x;
@@ -650,11 +269,13 @@ static void launch_dw(int dt, const void* dz, int64_t ldz, const void* x, int64_
   a.k = n;
   a.segs = 1;
   a.m = m;
+  a.am = mp;
   a.n = k;
+  a.bn = kp;
   a.y = dw;
   a.ws = ws;
   a.kz = sh.kz;
-  launch_product<true, true, false>(dt, a, sh, s);
+  launch_product(dt, a, DENSE_COLS, sh, s);
 }
 
 }  // namespace bcfft
@@ -666,42 +287,32 @@ extern "C" {
 int64_t bcfft_dense_workspace_bytes(int op, int64_t n_tokens, int64_t in_features, int64_t out_features, int dtype,
                                     int act) {
   if (!valid_dt(dtype) || !valid_sizes(n_tokens, in_features, out_features) || act < 0 || act > BCFFT_ACT_GELU) return -1;
+  if (op < BCFFT_DENSE_LINEAR || op > BCFFT_DENSE_GLU_BACKWARD) return -1;
   if (n_tokens == 0) return 0;
-  switch (op) {
-    case BCFFT_DENSE_LINEAR:
-      return partial_bytes(n_tokens, out_features, choose(n_tokens, out_features, ksteps(in_features, dtype), 1, true));
-    case BCFFT_DENSE_GLU:
-      return partial_bytes(n_tokens, 2 * out_features, choose(n_tokens, out_features, ksteps(in_features, dtype), 2, true));
-    case BCFFT_DENSE_LINEAR_BACKWARD: return backward_plan(n_tokens, in_features, out_features, dtype, 1, act).total;
-    case BCFFT_DENSE_GLU_BACKWARD: return backward_plan(n_tokens, in_features, out_features, dtype, 2, act).total;
-    default: return -1;
-  }
+  const int parts = op == BCFFT_DENSE_GLU || op == BCFFT_DENSE_GLU_BACKWARD ? 2 : 1;
+  if (op == BCFFT_DENSE_LINEAR || op == BCFFT_DENSE_GLU) return forward_plan(n_tokens, in_features, out_features, dtype, parts).total;
+  return backward_plan(n_tokens, in_features, out_features, dtype, parts, act).total;
 }
 
 int bcfft_dense_linear(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
                        int64_t out_features, const void* w, const void* bias, const void* residual, int64_t r_stride,
                        int act, void* y, float* z, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!valid_dt(dtype)) return BCFFT_ERR_DTYPE;
-  if (!valid_sizes(n_tokens, in_features, out_features) || x_stride < in_features || x_stride > (1 << 20) ||
+  if (!valid_sizes(n_tokens, in_features, out_features) || !valid_stride(x_stride, in_features) ||
       (residual && r_stride < out_features))
     return BCFFT_ERR_SHAPE;
   if (act < 0 || act > BCFFT_ACT_GELU) return BCFFT_ERR_ARG;
   if (n_tokens == 0) return BCFFT_OK;
   if (!x || !w || !y) return BCFFT_ERR_ARG;
   const int e = elem(dtype);
-  if (!aligned_to(x, e) || !aligned_to(w, e) || !aligned_to(bias, e) || !aligned_to(residual, e) || !aligned_to(y, e) ||
-      !aligned_to(z, 4) || !aligned_to(workspace, 16))
+  if (!aligned_to(x, 16) || !aligned_to(w, 16) || !aligned_stride(x_stride, n_tokens, in_features, dtype) ||
+      !aligned_to(bias, e) || !aligned_to(residual, e) || !aligned_to(y, e) || !aligned_to(z, 4) || !aligned_to(workspace, 16))
     return BCFFT_ERR_ALIGN;
-  Shape sh = choose(n_tokens, out_features, ksteps(in_features, dtype), 1, true);
-  const int64_t need = partial_bytes(n_tokens, out_features, sh);
-  if (need > 0 && (!workspace || workspace_bytes < need)) sh.kz = 1;
   DenseArgs a{};
   a.a[0] = x;
   a.b[0] = w;
   a.lda = x_stride;
-  a.ldb = in_features;
-  a.k = in_features;
-  a.segs = 1;
+  a.ldb = a.k = in_features;
   a.m = n_tokens;
   a.n = out_features;
   a.bias = bias;
@@ -710,81 +321,75 @@ int bcfft_dense_linear(const void* x, int dtype, int64_t n_tokens, int64_t x_str
   a.y = y;
   a.z = z;
   a.act = act;
-  a.ws = (float*)workspace;
-  a.kz = sh.kz;
-  launch_product<false, false, false>(dtype, a, sh, (hipStream_t)stream);
-  return record_launch_status();
+  return run_forward(dtype, a, nullptr, forward_plan(n_tokens, in_features, out_features, dtype, 1), workspace,
+                     workspace_bytes, (hipStream_t)stream);
 }
 
 int bcfft_dense_glu(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
                     int64_t out_features, const void* w_gate, const void* w_up, int act, void* h, float* gu,
                     void* workspace, int64_t workspace_bytes, void* stream) {
   if (!valid_dt(dtype)) return BCFFT_ERR_DTYPE;
-  if (!valid_sizes(n_tokens, in_features, out_features) || x_stride < in_features || x_stride > (1 << 20)) return BCFFT_ERR_SHAPE;
+  if (!valid_sizes(n_tokens, in_features, out_features) || !valid_stride(x_stride, in_features)) return BCFFT_ERR_SHAPE;
   if (act < 0 || act > BCFFT_ACT_GELU) return BCFFT_ERR_ARG;
   if (n_tokens == 0) return BCFFT_OK;
   if (!x || !w_gate || !w_up || !h) return BCFFT_ERR_ARG;
   const int e = elem(dtype);
-  if (!aligned_to(x, e) || !aligned_to(w_gate, e) || !aligned_to(w_up, e) || !aligned_to(h, e) || !aligned_to(gu, 4) ||
+  if (!aligned_to(x, 16) || !aligned_to(w_gate, 16) || !aligned_to(w_up, 16) ||
+      !aligned_stride(x_stride, n_tokens, in_features, dtype) || !aligned_to(h, e) || !aligned_to(gu, 4) ||
       !aligned_to(workspace, 16))
     return BCFFT_ERR_ALIGN;
-  Shape sh = choose(n_tokens, out_features, ksteps(in_features, dtype), 2, true);
-  const int64_t need = partial_bytes(n_tokens, 2 * out_features, sh);
-  if (need > 0 && (!workspace || workspace_bytes < need)) sh.kz = 1;
   DenseArgs a{};
   a.a[0] = x;
   a.b[0] = w_gate;
-  a.b[1] = w_up;
   a.lda = x_stride;
-  a.ldb = in_features;
-  a.k = in_features;
-  a.segs = 1;
+  a.ldb = a.k = in_features;
   a.m = n_tokens;
   a.n = out_features;
   a.y = h;
   a.z = gu;
   a.act = act;
-  a.ws = (float*)workspace;
-  a.kz = sh.kz;
-  launch_product<false, false, true>(dtype, a, sh, (hipStream_t)stream);
-  return record_launch_status();
+  return run_forward(dtype, a, w_up, forward_plan(n_tokens, in_features, out_features, dtype, 2), workspace,
+                     workspace_bytes, (hipStream_t)stream);
 }
 
 int bcfft_dense_linear_backward(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
                                 int64_t out_features, const void* w, const void* dy, int64_t dy_stride, const float* z,
                                 int act, void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes,
                                 void* stream) {
+  const int64_t n = n_tokens, k = in_features, m = out_features;
   if (!valid_dt(dtype)) return BCFFT_ERR_DTYPE;
-  if (!valid_sizes(n_tokens, in_features, out_features) || x_stride < in_features || x_stride > (1 << 20) ||
-      dy_stride < out_features || dy_stride > (1 << 20))
-    return BCFFT_ERR_SHAPE;
-  if (act < 0 || act > BCFFT_ACT_GELU || n_tokens == 0) return BCFFT_ERR_ARG;
+  if (!valid_sizes(n, k, m) || !valid_stride(x_stride, k) || !valid_stride(dy_stride, m)) return BCFFT_ERR_SHAPE;
+  if (act < 0 || act > BCFFT_ACT_GELU || n == 0) return BCFFT_ERR_ARG;
   if (!dy || (act != BCFFT_ACT_NONE && !z) || (dx && !w) || (dw && !x)) return BCFFT_ERR_ARG;
   const int e = elem(dtype);
-  if (!aligned_to(x, e) || !aligned_to(w, e) || !aligned_to(dy, e) || !aligned_to(z, 4) || !aligned_to(dx, e) ||
+  if ((dw && (!aligned_to(x, 16) || !aligned_stride(x_stride, n, k, dtype))) || (dx && !aligned_to(w, 16)) ||
+      !aligned_to(dy, 16) || !aligned_stride(dy_stride, n, m, dtype) || !aligned_to(z, 4) || !aligned_to(dx, e) ||
       !aligned_to(dw, e) || !aligned_to(db, e) || !aligned_to(workspace, 16))
     return BCFFT_ERR_ALIGN;
-  const BackwardPlan p = backward_plan(n_tokens, in_features, out_features, dtype, 1, act);
+  const BackwardPlan p = backward_plan(n, k, m, dtype, 1, act);
   if (p.total > 0 && (!workspace || workspace_bytes < p.total)) return BCFFT_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
-  void* dz = act != BCFFT_ACT_NONE ? ws : nullptr;
+  void* dz = p.dz_bytes ? ws : nullptr;                // dy itself where it needs neither slope nor padding
   float* part = (float*)(ws + p.dz_bytes);
-  float* sums = (float*)(ws + p.dz_bytes + p.part_bytes);
-  if (dz || db) {
-    const DzArgs d{dy, dy_stride, dz ? z : nullptr, (dx || dw) ? dz : nullptr, db ? part : nullptr, n_tokens, out_features, act};
+  ws += p.dz_bytes + p.part_bytes;
+  const int64_t mp = padded(m, dtype), kp = padded(k, dtype);
+  if ((dz && (dx || dw)) || db) {
+    const DzArgs d{dy, dy_stride, act != BCFFT_ACT_NONE ? z : nullptr, dx || dw ? dz : nullptr, mp, db ? part : nullptr,
+                   n, m, act};
     by_dtype(dtype, [&](auto dt) {
-      hipLaunchKernelGGL(bc_dense_dz_kernel<dt.value>, dim3((unsigned)p.slices, (unsigned)((out_features + 1023) / 1024)),
-                         dim3(256), 0, s, d);
+      hipLaunchKernelGGL(bc_dense_dz_kernel<dt.value>, dim3((unsigned)p.slices, (unsigned)((m + 255) / 256)), dim3(256), 0, s, d);
       if (db)
-        hipLaunchKernelGGL(bc_dense_db_kernel<dt.value>, dim3((unsigned)((out_features + 255) / 256)), dim3(256), 0, s, part,
-                           p.slices, out_features, db);
+        hipLaunchKernelGGL(bc_dense_db_kernel<dt.value>, dim3((unsigned)((m + 31) / 32)), dim3(256), 0, s, part, p.slices, m, db);
     });
   }
   const void* g = dz ? dz : dy;
-  const int64_t ldg = dz ? out_features : dy_stride;
-  if (dx) launch_dx(dtype, g, ldg, w, nullptr, n_tokens, in_features, out_features, p.dx, dx, sums, s);
-  if (dw) launch_dw(dtype, g, ldg, x, x_stride, n_tokens, in_features, out_features, p.dw, dw, sums, s);
+  const int64_t ldg = dz ? mp : dy_stride;
+  const bool packed = p.pack_bytes > 0;
+  const void* wp = packed && dx ? pack(dtype, w, k, m, k, ws, s) : w;
+  const void* xp = packed && dw ? pack(dtype, x, x_stride, n, k, ws, s) : x;
+  if (dx) launch_dx(dtype, g, ldg, 0, wp, nullptr, n, k, packed ? kp : k, m, p.dx, dx, (float*)ws, s);
+  if (dw) launch_dw(dtype, g, ldg, dz ? mp : m, xp, packed ? kp : x_stride, packed ? kp : k, n, k, m, p.dw, dw, (float*)ws, s);
   return record_launch_status();
 }
 
@@ -792,27 +397,39 @@ int bcfft_dense_glu_backward(const void* x, int dtype, int64_t n_tokens, int64_t
                              int64_t out_features, const void* w_gate, const void* w_up, const void* dh,
                              int64_t dh_stride, const float* gu, int act, void* dx, void* dw, void* workspace,
                              int64_t workspace_bytes, void* stream) {
+  const int64_t n = n_tokens, k = in_features, m = out_features;
   if (!valid_dt(dtype)) return BCFFT_ERR_DTYPE;
-  if (!valid_sizes(n_tokens, in_features, out_features) || 2 * out_features > (1 << 20) || x_stride < in_features ||
-      x_stride > (1 << 20) || dh_stride < out_features)
-    return BCFFT_ERR_SHAPE;
-  if (act < 0 || act > BCFFT_ACT_GELU || n_tokens == 0) return BCFFT_ERR_ARG;
+  if (!valid_sizes(n, k, m) || 2 * m > (1 << 20) || !valid_stride(x_stride, k) || dh_stride < m) return BCFFT_ERR_SHAPE;
+  if (act < 0 || act > BCFFT_ACT_GELU || n == 0) return BCFFT_ERR_ARG;
   if (!dh || !gu || (dx && (!w_gate || !w_up)) || (dw && !x)) return BCFFT_ERR_ARG;
   const int e = elem(dtype);
-  if (!aligned_to(x, e) || !aligned_to(w_gate, e) || !aligned_to(w_up, e) || !aligned_to(dh, e) || !aligned_to(gu, 4) ||
+  if ((dw && (!aligned_to(x, 16) || !aligned_stride(x_stride, n, k, dtype))) ||
+      (dx && (!aligned_to(w_gate, 16) || !aligned_to(w_up, 16))) || !aligned_to(dh, e) || !aligned_to(gu, 4) ||
       !aligned_to(dx, e) || !aligned_to(dw, e) || !aligned_to(workspace, 16))
     return BCFFT_ERR_ALIGN;
-  const BackwardPlan p = backward_plan(n_tokens, in_features, out_features, dtype, 2, act);
+  const BackwardPlan p = backward_plan(n, k, m, dtype, 2, act);
   if (!workspace || workspace_bytes < p.total) return BCFFT_ERR_ARG;
+  if (!dx && !dw) return BCFFT_OK;
   hipStream_t s = (hipStream_t)stream;
-  char* ws = (char*)workspace;
-  float* sums = (float*)(ws + p.dz_bytes);
-  const DzArgs d{dh, dh_stride, gu, ws, nullptr, n_tokens, out_features, act};
-  const int64_t quads = (out_features + 3) / 4 * n_tokens;
+  char* dz = (char*)workspace;
+  char* ws = dz + p.dz_bytes + p.part_bytes;
+  const int64_t mp = padded(m, dtype), kp = padded(k, dtype);
+  const DzArgs d{dh, dh_stride, gu, dz, 2 * mp, nullptr, n, m, act};
+  const int64_t quads = (m + 3) / 4 * n;
   const unsigned blocks = (unsigned)((quads + 255) / 256 < 65536 ? (quads + 255) / 256 : 65536);
   by_dtype(dtype, [&](auto dt) { hipLaunchKernelGGL(bc_dense_dgu_kernel<dt.value>, dim3(blocks), dim3(256), 0, s, d); });
-  if (dx) launch_dx(dtype, ws, 2 * out_features, w_gate, w_up, n_tokens, in_features, out_features, p.dx, dx, sums, s);
-  if (dw) launch_dw(dtype, ws, 2 * out_features, x, x_stride, n_tokens, in_features, 2 * out_features, p.dw, dw, sums, s);
+  const bool packed = p.pack_bytes > 0;
+  const void* wgp = packed && dx ? pack(dtype, w_gate, k, m, k, ws, s) : w_gate;
+  const void* wup = packed && dx ? pack(dtype, w_up, k, m, k, ws, s) : w_up;
+  const void* xp = packed && dw ? pack(dtype, x, x_stride, n, k, ws, s) : x;
+  const int64_t ldx = packed ? kp : x_stride, kr = packed ? kp : k;
+  if (dx) launch_dx(dtype, dz, 2 * mp, mp, wgp, wup, n, k, kr, m, p.dx, dx, (float*)ws, s);
+  if (dw && mp == m) {
+    launch_dw(dtype, dz, 2 * mp, 2 * mp, xp, ldx, kr, n, k, 2 * m, p.dw, dw, (float*)ws, s);
+  } else if (dw) {
+    launch_dw(dtype, dz, 2 * mp, mp, xp, ldx, kr, n, k, m, p.dw, dw, (float*)ws, s);
+    launch_dw(dtype, dz + mp * e, 2 * mp, mp, xp, ldx, kr, n, k, m, p.dw, (char*)dw + m * k * e, (float*)ws, s);
+  }
   return record_launch_status();
 }
 

@@ -1,0 +1,8 @@
+// bcfft_dense_f16.hip — the dense products of fp16 operands (kernels: bcfft_dense_tile.h, bcfft_dense_launch.h).
+#include "bcfft_dense_launch.h"
+
+namespace bcfft {
+void launch_product_f16(const DenseArgs& a, DenseLayout layout, Shape sh, hipStream_t s) {
+  launch_product_dt<BCFFT_F16>(a, layout, sh, s);
+}
+}  // namespace bcfft

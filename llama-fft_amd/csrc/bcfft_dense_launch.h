@@ -1,0 +1,153 @@
+// bcfft_dense_launch.h — the dense products' kernels of one dtype and their launch, included by
+// bcfft_dense_{f32,f16,bf16}.hip (one translation unit each).
+#pragma once
+#include "bcfft_dense_tile.h"
+
+namespace bcfft {
+
+// sums the slices of a split k in order and finishes the output
+template <int DT, bool GLU>
+__global__ __launch_bounds__(256) void bc_dense_finish_kernel(DenseArgs a) {
+  const int64_t quads = (a.n + 3) / 4, total = quads * a.m;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
+    const int64_t m = q / quads, n = (q - m * quads) * 4;
+    const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
+    f32x4 g = load_partials(a, m, n, cnt);
+    if constexpr (GLU) finish_glu<DT>(a, m, n, g, load_partials(a, m, a.n + n, cnt), cnt);
+    else finish_linear<DT>(a, m, n, g, cnt);
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+// Up to 16 MT rows of x (decode): bound by the weights' single read. A workgroup takes 16 rows of W (and 16
+// of the other weight, GLU), its KW waves a part of k each, straight from memory into the fragments; x comes
+// out of L2. The waves' sums meet in LDS.
+template <int DT, int MT, int KW, bool GLU>
+__global__ __launch_bounds__(64 * KW) void bc_dense_rows_kernel(DenseArgs a) {
+  constexpr int E = DT == BCFFT_F32 ? 4 : 2, EPC = 16 / E, BK = 128 / E, NB = GLU ? 2 : 1;
+  constexpr int UNROLL = 4;
+  __shared__ f32x4 part[KW][NB * MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l = lane & 15;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t wrow = n0 + l < a.n ? n0 + l : a.n - 1;       // repeated rows are not stored
+  const char* pw[NB];
+#pragma unroll
+  for (int s = 0; s < NB; ++s) pw[s] = (const char*)a.b[s] + wrow * a.ldb * E;
+  const char* px[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) px[i] = (const char*)a.a[0] + (16 * i + l < a.m ? 16 * i + l : a.m - 1) * a.lda * E;
+  const int64_t tiles = (a.k + BK - 1) / BK;
+  const int64_t t0 = tiles * wave / KW, t1 = tiles * (wave + 1) / KW;
+
+  f32x4 acc[NB][MT];
+#pragma unroll
+  for (int s = 0; s < NB; ++s)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[s][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto load = [&](const char* p, int64_t k) {          // 16 bytes of k, whatever the address
+    const Unaligned16<E> u = *reinterpret_cast<const Unaligned16<E>*>(p + k * E);
+    return make_uint4(u.w[0], u.w[1], u.w[2], u.w[3]);
+  };
+  auto step = [&](const uint4 (&w)[NB], const uint4 (&x)[MT]) {
+#pragma unroll
+    for (int s = 0; s < NB; ++s)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[s][i] = mma<DT>(w[s], x[i], acc[s][i]);
+  };
+  int64_t t = t0;
+  for (; t + UNROLL <= t1 && (t + UNROLL) * BK <= a.k; t += UNROLL) {
+    uint4 w[UNROLL][2][NB], x[UNROLL][2][MT];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const int64_t k = (t + u) * BK + (g + 4 * kk) * EPC;
+#pragma unroll
+        for (int s = 0; s < NB; ++s) w[u][kk][s] = load(pw[s], k);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[u][kk][i] = load(px[i], k);
+      }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) step(w[u][kk], x[u][kk]);
+  }
+  for (; t < t1; ++t) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const int64_t k = t * BK + (g + 4 * kk) * EPC;
+      uint4 w[NB], x[MT];
+#pragma unroll
+      for (int s = 0; s < NB; ++s) w[s] = load_part<E>(pw[s], k, a.k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) x[i] = load_part<E>(px[i], k, a.k);
+      step(w, x);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < NB; ++s)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[wave][s * MT + i][lane] = acc[s][i];
+  __syncthreads();
+  for (int i = wave; i < MT; i += KW) {
+    const int64_t m = 16 * i + l, n = n0 + 4 * g;
+    if (m >= a.m || n >= a.n) continue;
+    f32x4 v[NB];
+#pragma unroll
+    for (int s = 0; s < NB; ++s) {
+      v[s] = part[0][s * MT + i][lane];
+#pragma unroll
+      for (int w = 1; w < KW; ++w) v[s] += part[w][s * MT + i][lane];
+    }
+    const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
+    if constexpr (GLU) finish_glu<DT>(a, m, n, v[0], v[NB - 1], cnt);
+    else finish_linear<DT>(a, m, n, v[0], cnt);
+  }
+}
+
+template <int DT, bool CA, bool CB, int BM, int BN, int WM, int WN, int RA, int RB, bool GLU>
+static void launch_tile(const DenseArgs& a, hipStream_t s) {
+  constexpr int BR = GLU ? BN / 2 : BN;
+  constexpr unsigned lds = (RA * BM + RB * BN) * 128;
+  auto kern = bc_dense_tile_kernel<DT, CA, CB, BM, BN, WM, WN, RA, RB, GLU>;
+  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  const unsigned tiles = (unsigned)(((a.m + BM - 1) / BM) * ((a.n + BR - 1) / BR));
+  hipLaunchKernelGGL(kern, dim3(tiles, (unsigned)a.kz), dim3(64 * WM * WN), lds, s, a);
+}
+
+template <int DT, bool CA, bool CB, bool GLU>
+static void launch_tiles(const DenseArgs& a, int kind, hipStream_t s) {
+  if (kind == 1) launch_tile<DT, CA, CB, 128, 128, 2, 2, 3, 2, GLU>(a, s);
+  else if (kind == 2) launch_tile<DT, CA, CB, 256, 128, 4, 2, 3, 3, GLU>(a, s);
+  else launch_tile<DT, CA, CB, 256, 256, 2, 4, 3, 2, GLU>(a, s);
+  if (a.kz > 1) {
+    const int64_t quads = (a.n + 3) / 4 * a.m;
+    const unsigned blocks = (unsigned)((quads + 255) / 256 < 16384 ? (quads + 255) / 256 : 16384);
+    hipLaunchKernelGGL((bc_dense_finish_kernel<DT, GLU>), dim3(blocks), dim3(256), 0, s, a);
+  }
+}
+
+template <int DT, bool GLU>
+static void launch_rows(const DenseArgs& a, hipStream_t s) {
+  const unsigned groups = (unsigned)((a.n + 15) / 16);
+  auto go = [&](auto mt, auto kw) {
+    hipLaunchKernelGGL((bc_dense_rows_kernel<DT, mt.value, kw.value, GLU>), dim3(groups), dim3(64 * kw.value), 0, s, a);
+  };
+  using std::integral_constant;
+  if (a.m <= 16 && groups <= 512) go(integral_constant<int, 1>(), integral_constant<int, 8>());
+  else if (a.m <= 16) go(integral_constant<int, 1>(), integral_constant<int, 4>());
+  else if (groups <= 512) go(integral_constant<int, 2>(), integral_constant<int, 8>());
+  else go(integral_constant<int, 2>(), integral_constant<int, 4>());
+}
+
+template <int DT>
+static void launch_product_dt(const DenseArgs& a, DenseLayout layout, Shape sh, hipStream_t s) {
+  switch (layout) {
+    case DENSE_ROWS: return sh.kind == 0 ? launch_rows<DT, false>(a, s) : launch_tiles<DT, false, false, false>(a, sh.kind, s);
+    case DENSE_GLU: return sh.kind == 0 ? launch_rows<DT, true>(a, s) : launch_tiles<DT, false, false, true>(a, sh.kind, s);
+    case DENSE_ROWS_COLS: return launch_tiles<DT, false, true, false>(a, sh.kind, s);
+    case DENSE_COLS: return launch_tiles<DT, true, true, false>(a, sh.kind, s);
+  }
+}
+
+}  // namespace bcfft
