@@ -114,6 +114,7 @@ _native = None
 # the operators' handles (OpOverload), looked up once: torch.ops attribute access costs ~1 us a call
 NATIVE_FORWARD = None
 NATIVE_FORWARD_GLU = None
+NATIVE_OPS = {}             # further operators by name (csrc/bcfft_torch_ops.cpp)
 _lock = threading.RLock()
 # torch.ops.bcfft_native (csrc/bcfft_torch.cpp): the C++ operators over this ABI, built next to it
 TORCH_OP_PATH = os.path.join(os.path.dirname(LIB_PATH), "libbcfft_torch.so")
@@ -143,8 +144,8 @@ def load() -> ctypes.CDLL:
 
 
 def native_op() -> bool:
-    """True once torch.ops.bcfft_native is loaded: the hot forward / forward_glu calls then go
-    through one C++ dispatcher op (argument checks, allocation, stream lookup and the launch in
+    """True once torch.ops.bcfft_native is loaded: the hot forward / forward_glu calls, the dense
+    projections and the distillation operators then go through one C++ dispatcher op (argument checks, allocation, stream lookup and the launch in
     C++) instead of ctypes. False when that library is not built, when BCFFT_NATIVE_OP=0, when
     BCFFT_LIB_PATH names another engine library (the operators link the in-tree libbcfft.so), or
     when the library is present but does not load (e.g. built against another torch: undefined
@@ -168,6 +169,8 @@ def native_op() -> bool:
                 if ok:
                     NATIVE_FORWARD = torch.ops.bcfft_native.forward.default
                     NATIVE_FORWARD_GLU = torch.ops.bcfft_native.forward_glu.default
+                    for name in ("dense_linear", "dense_glu", "topk_logits", "topk_kl", "topk_kl_grad"):
+                        NATIVE_OPS[name] = getattr(torch.ops.bcfft_native, name).default
                 _native = ok
     return _native
 

@@ -75,6 +75,10 @@ def _check(what: str, x: torch.Tensor, weights, vectors, activation) -> int:
             raise TypeError(f"{what}: {name} is {t.dtype} but x is {x.dtype}; all operands share one dtype")
         if t is not None and t.device != x.device:
             raise ValueError(f"{what}: {name} is on {t.device} but x is on {x.device}; move it to x's device")
+    return _activation(what, activation)
+
+
+def _activation(what: str, activation) -> int:
     if activation not in _lib.ACTIVATIONS:
         raise ValueError(f"{what}: activation {activation!r}, expected one of {list(_lib.ACTIVATIONS)}")
     return _lib.ACTIVATIONS[activation]
@@ -150,6 +154,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     "relu", "silu" or "gelu" (exact). fp32 accumulation, one rounding. Up to 32 rows run the weight-streaming
     kernel. The gradient of an activation's input is rounded once to the dtype before the two products that
     read it; bias gradients sum the unrounded values."""
+    if _lib.native_op():                         # the same call as one C++ op (csrc/bcfft_torch_ops.cpp)
+        return _lib.NATIVE_OPS["dense_linear"](x, weight, bias, residual, _activation("bcfft.dense.linear", activation))
     lead = x.shape[:-1]
     act = _check("bcfft.dense.linear", x, [("weight", weight)],
                  [("bias", bias, weight.shape[:1]), ("residual", residual, lead + weight.shape[:1])], activation)
@@ -218,6 +224,8 @@ def glu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation
     x (..., in_features), w_gate and w_up (out_features, in_features), all float32, float16 or bfloat16
     alike. activation: "silu" (LLaMA), "gelu" (exact), "relu" or None. fp32 up to h's one rounding; the
     backward rounds dg and du once to the dtype before the products that read them."""
+    if _lib.native_op():
+        return _lib.NATIVE_OPS["dense_glu"](x, w_gate, w_up, _activation("bcfft.dense.glu", activation))
     act = _check("bcfft.dense.glu", x, [("w_gate", w_gate), ("w_up", w_up)], [], activation)
     if 2 * w_gate.shape[0] > MAX_FEATURES:
         raise ValueError(f"bcfft.dense.glu: out_features = {w_gate.shape[0]}, at most {MAX_FEATURES // 2}")

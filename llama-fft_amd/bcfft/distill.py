@@ -57,6 +57,8 @@ def topk_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     logits come lowest index first, NaN before everything. indices (..., k) int32. rest (...) float32 =
     log(sum of exp(logit / temperature) over the logits not taken), -inf where none is left.
     1 <= k <= min(V, 1024). Not differentiable (the teacher is a constant)."""
+    if _lib.native_op():                         # the same call as one C++ op (csrc/bcfft_torch_ops.cpp)
+        return _lib.NATIVE_OPS["topk_logits"](logits, k, temperature)
     what = "bcfft.distill.topk_logits"
     _lib.require_device(logits, what)
     x = _rows(logits.detach(), what)
@@ -173,6 +175,8 @@ def topk_kl(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, *
 
     The gradient comes in logits' dtype; teacher side and weights are constants. To capture a training
     step into a graph, capture forward and backward together."""
+    if _lib.native_op():
+        return _lib.NATIVE_OPS["topk_kl"](logits, values, indices, rest, weight, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
         _lib.require_device(logits, "bcfft.distill.topk_kl")
         return _TopKKL.apply(logits, values, indices, rest, weight, temperature)
@@ -185,6 +189,8 @@ def topk_kl_grad(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
     """(loss, dlogits) in one launch that reads the logits once: topk_kl's losses and the gradient of
     their SUM with respect to the logits, in logits' dtype, contiguous. For a mean give weight = 1 / rows.
     `logits.backward(dlogits)` carries it into the model. Same operands as topk_kl; not recorded by autograd."""
+    if _lib.native_op():
+        return _lib.NATIVE_OPS["topk_kl_grad"](logits, values, indices, rest, weight, temperature)
     op = _Operands(logits, values, indices, rest, weight, temperature, "bcfft.distill.topk_kl_grad")
     loss, _, g = op.forward(stats=False, grad=True)
     return loss.view(logits.shape[:-1]), g.view(logits.shape)

@@ -370,3 +370,36 @@ def test_refusals(dev):
         dense.linear(x, w.cpu())
     with pytest.raises(ValueError, match="scalar"):
         dense.linear(torch.tensor(1.0, device=dev), w)
+
+
+def test_ctypes_path_is_identical(dev, monkeypatch):
+    """The Python / ctypes path and the C++ operators run the same kernels: equal bits, forward and backward."""
+    from bcfft import _lib, dense
+    assert _lib.native_op(), "libbcfft_torch.so not loaded"
+    for n, k, m, dt in ((5, 72, 24, torch.float16), (200, 1000, 130, torch.bfloat16), (0, 64, 32, torch.float32), (40, 129, 33, torch.float32)):
+        x, w, wu = (rand(dev, *s, dt=dt, seed=71 + i, scale=0.1) for i, s in enumerate(((n, k), (m, k), (m, k))))
+        b, r, dy = (rand(dev, *s, dt=dt, seed=75 + i) for i, s in enumerate(((m,), (n, m), (n, m))))
+
+        def both():
+            out = []
+            ins = [t.clone().requires_grad_() for t in (x, w, b, r)]
+            y = dense.linear(ins[0], ins[1], ins[2], activation="gelu", residual=ins[3])
+            out += [y.detach(), *torch.autograd.grad(y, ins, dy)]
+            ins = [t.clone().requires_grad_() for t in (x, w, wu)]
+            h = dense.glu(*ins)
+            return out + [h.detach(), *torch.autograd.grad(h, ins, dy), dense.linear(x, w), dense.glu(x, w, wu)]
+        native = both()
+        with monkeypatch.context() as mp:
+            mp.setattr(_lib, "_native", False)
+            other = both()
+        assert all(torch.equal(p, q) for p, q in zip(native, other))
+
+
+def test_second_derivative_is_refused(dev):
+    from bcfft import dense
+    x, w, wu = (rand(dev, *s, dt=torch.float32, seed=81).requires_grad_() for s in ((4, 16), (8, 16), (8, 16)))
+    for y in (dense.linear(x, w, activation="gelu"), dense.glu(x, w, wu)):
+        up = torch.ones_like(y).requires_grad_()
+        (dx,) = torch.autograd.grad(y, x, up, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            dx.sum().backward()

@@ -378,3 +378,26 @@ def test_refusals(dev):
         distill.topk_kl(s, values.requires_grad_(), indices)
     with pytest.raises(ValueError, match="vocabulary"):
         distill.topk_kl(torch.zeros(1, (1 << 18) + 1, device=dev), values[:1].detach(), indices[:1])
+
+
+def test_ctypes_path_is_identical(dev, monkeypatch):
+    """The Python / ctypes path and the C++ operators run the same kernels: equal bits."""
+    from bcfft import _lib, distill
+    assert _lib.native_op(), "libbcfft_torch.so not loaded"
+    for shape, k, idx in (((3, 4, 501), 7, torch.int64), ((6, 32000), 64, torch.int32), ((0, 90), 5, torch.int32)):
+        s = logits_of(max(1, int(torch.tensor(shape[:-1]).prod())), shape[-1], torch.float16, seed=31)
+        s = s[:int(torch.tensor(shape[:-1]).prod())].reshape(shape).to(dev)
+        w = torch.rand(shape[:-1], device=dev)
+
+        def all_of():
+            values, indices, rest = distill.topk_logits(s.flip(-1), k, 1.5)
+            x = s.clone().requires_grad_()
+            loss = distill.topk_kl(x, values, indices.to(idx), rest=rest, weight=w, temperature=1.5)
+            (g,) = torch.autograd.grad(loss, x, torch.ones_like(loss) * 0.5)
+            return [values, indices, rest, loss.detach(), g,
+                    *distill.topk_kl_grad(s, values, indices.to(idx), rest=rest, weight=w.double(), temperature=1.5)]
+        native = all_of()
+        with monkeypatch.context() as mp:
+            mp.setattr(_lib, "_native", False)
+            other = all_of()
+        assert all(p.shape == q.shape and p.dtype == q.dtype and torch.equal(p, q) for p, q in zip(native, other))
