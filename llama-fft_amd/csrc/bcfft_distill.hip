@@ -10,14 +10,14 @@
 //   dloss/ds_v = (w g / T) (q_v - sum_{j: i_j = v} P_j)   for v among the i_j
 //                (w g / T) (q_v - P_rest q_v / q_rest)    else
 //
-// One workgroup per row. Bound by HBM: a row is read once, into registers (HOLD 16-byte pieces per
-// thread, up to 131072 16-bit logits), and every further pass (maxima, sums, gradients) runs on them;
-// longer rows are read again, out of L2 / the memory-side cache. A 1024-thread workgroup may use 128
-// VGPRs per thread, 64 of them hold the row, so two workgroups of 512 threads (32000 16-bit logits)
-// share a CU and one's arithmetic runs under the other's loads.
+// One workgroup per row. A row is read once, into registers (HOLD 16-byte pieces per thread, up to 131072
+// 16-bit logits); longer rows are read again, out of L2 / the memory-side cache. The floor is HBM: 3.2 us a
+// CU for a row of 32000 16-bit logits read, 6.4 us read and written back. A CU serves 64 lane operations a
+// clock (an exponential counts four), so a row's floor allows 14 (28) of them per logit: what the passes
+// cost is counted beside them, and exponentials that the gradient needs again stay in registers.
 //
-// The loss is a small difference of logarithms: a thread's part of a sum is kept in fp32 (at most a few
-// hundred terms of one sign), the sums over threads, the teacher's softmax and the logarithms in fp64.
+// The loss is a small difference of logarithms: a thread's part of a sum is kept in fp32 (at most 128 terms
+// of one sign), the sums over threads, the teacher's softmax and the logarithms in fp64.
 #include "bcfft_device.h"
 
 #include <type_traits>
@@ -25,18 +25,27 @@
 namespace bcfft {
 
 constexpr int TOPK_MAX = 1024;          // entries per row
-constexpr int TOPK_CAND = 2048;         // candidates ranked in LDS
 constexpr int DISTILL_VOCAB_MAX = 1 << 18;   // the entries' bitmap: 32 KB of LDS
 
-// exp(x / T) as exp2(x c + x lo): c + lo = log2(e) / T to 48 bits, so the constant's own rounding
-// (up to 3e-8 relative, times x: the same sign in every term) does not shift the whole sum.
-// c is rounded down and lo > 0: for x = -inf both products are -inf, never inf - inf.
+// exp((v - ref) / T) as exp2(v c + v lo + b), b = -ref c rounded: c + lo = log2(e) / T to 48 bits, so the
+// constant's own rounding (up to 3e-8 relative, times v: the same sign in every term) does not shift the
+// sum; b's rounding multiplies every term alike and is taken out of the sums in fp64 (drift).
+// c is rounded down and lo > 0: for v = -inf both products are -inf, never inf - inf.
 struct ExpScale {
   float c, lo;
 };
-__device__ __forceinline__ float exp_scaled(float x, ExpScale e) {
-  return __builtin_amdgcn_exp2f(fmaf(x, e.c, x * e.lo));
+__device__ __forceinline__ float exp_at(float v, ExpScale e, float b) {
+  return __builtin_amdgcn_exp2f(fmaf(v, e.lo, fmaf(v, e.c, b)));
 }
+// the same without lo: the constant's rounding is taken out at ref alone, which leaves it times the distance
+// from ref (at most as much as the argument's own rounding)
+__device__ __forceinline__ float exp_near(float v, ExpScale e, float b) { return __builtin_amdgcn_exp2f(fmaf(v, e.c, b)); }
+__device__ __forceinline__ float exp_base(float ref, ExpScale e) { return -ref * e.c; }
+// log2 of what exp_at's (drift_near: at v = ref, exp_near's) values are too large by
+__device__ __forceinline__ double drift(float ref, ExpScale e, float b) {
+  return (double)b + (double)ref * ((double)e.c + (double)e.lo);
+}
+__device__ __forceinline__ double drift_near(float ref, ExpScale e, float b) { return (double)b + (double)ref * (double)e.c; }
 
 template <int DT> struct RowType {
   static constexpr int VEC = 8;        // elements per 16 bytes
@@ -142,6 +151,15 @@ struct MaxOp {
 struct SumOp {
   template <class T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
 };
+// the waves' results, joined by every wave for itself (lane i takes wave i's: one value per thread, where a
+// loop over them would hold all)
+template <int NT, class T, class OP>
+__device__ __forceinline__ T across_waves(const T* red, OP op) {
+  T v = red[threadIdx.x & (NT / 64 - 1)];
+#pragma unroll
+  for (int d = NT / 128; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
+  return v;
+}
 // every thread gets the result, added up in a fixed order; `red` holds NT / 64 values and is free
 // again after the caller's next barrier
 template <int NT, class T, class OP>
@@ -150,10 +168,7 @@ __device__ __forceinline__ T block_reduce(T v, T* red, OP op) {
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  T r = red[0];
-#pragma unroll
-  for (int i = 1; i < NT / 64; ++i) r = op(r, red[i]);
-  return r;
+  return across_waves<NT>(red, op);
 }
 
 // ------------------------------------------------------------------ the teacher's top logits
@@ -169,21 +184,26 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 1. Each thread's largest key; the k-th largest of these NT keys bounds the k-th largest element from
-//    below (k threads hold at least one element that large each), and hardly more than k elements
-//    reach it (74 for k = 64 of 256 threads, evenly spread). Its upper 16 bits are enough.
-// 2. The elements at or above the bound go to LDS; each counts the candidates above it: its rank is its
-//    place in the output. Ranks depend on keys alone, so the order of arrival does not matter.
-// 3. The others' maximum and sum give rest.
+// 1. Each thread's largest logit; the k-th largest of these NT bounds the k-th largest element from below (k
+//    threads hold at least one that large each), and hardly more than k elements reach it (74 for k = 64
+//    of 256 threads, evenly spread). Its upper 16 bits are enough.                   1.5 operations a logit
+// 2. The elements at or above the bound go to LDS, the others' exponentials relative to it are summed.    9
+// 3. Each candidate counts the candidates above it: its rank is its place in the output. Ranks depend on
+//    keys alone, so the order of arrival does not matter.
 // If more than TOPK_CAND elements reach the bound (long runs of equal logits), the k-th key itself is
-// found bit by bit, by counting over the whole row.
+// found bit by bit, by counting over the whole row; if the sum under the bound vanishes in fp32 (a gap of
+// 45 T below the bound), the others' own maximum takes the bound's place as its reference.
 template <int DT, int NT, int HOLD>
-__global__ __launch_bounds__(NT) void bc_topk_logits_kernel(const void* __restrict__ logits, int64_t vocab,
+__global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(const void* __restrict__ logits, int64_t vocab,
                                                             int64_t row_stride, int k, ExpScale es, double inv_t,
                                                             void* __restrict__ values, int32_t* __restrict__ indices,
                                                             float* __restrict__ rest) {
   constexpr int E = DT == BCFFT_F32 ? 4 : 2;
-  __shared__ uint64_t cand[TOPK_CAND];
+  constexpr int TOPK_CAND = NT == 256 ? 1024 : 2048;     // candidates ranked in LDS (k <= NT)
+  constexpr int VEC = RowType<DT>::VEC, CHUNK = HOLD > 0 ? 64 / VEC : 1;    // pieces per 64-bit mask
+  __shared__ int at_s[TOPK_CAND];        // the candidates: indices, as they come
+  __shared__ uint64_t cand[TOPK_CAND];   // their keys
+  __shared__ uint32_t raw[TOPK_CAND];    // their logits as they stand in the row
   __shared__ float left[TOPK_CAND];
   __shared__ uint32_t tmax[NT];
   __shared__ uint32_t redu[NT / 64];
@@ -196,14 +216,15 @@ __global__ __launch_bounds__(NT) void bc_topk_logits_kernel(const void* __restri
   Row<DT, NT, HOLD> r;
   r.open(row, vocab);
 
-  uint32_t best = 0;                     // below every key of a number
+  float best = -INFINITY;                // NaN passes it by: it still is a candidate below
+  bool any = false;
   r.each([&](int, auto& v) {
-    for (float x : v) {
-      const uint32_t key = order_key(x);
-      best = key > best ? key : best;
-    }
+    any = true;
+#pragma unroll
+    for (int j = 0; j + 1 < count_of<decltype(v)>; j += 2) best = fmaxf(fmaxf(best, v[j]), v[j + 1]);
+    if constexpr (count_of<decltype(v)> == 1) best = fmaxf(best, v[0]);
   });
-  tmax[tid] = best;
+  tmax[tid] = any ? order_key(best) : 0;   // 0 is below every key of a number
   if (tid == 0) count = 0;
   __syncthreads();
   if (tid < 64) {                        // largest b with k thread maxima whose upper halves reach it
@@ -221,92 +242,156 @@ __global__ __launch_bounds__(NT) void bc_topk_logits_kernel(const void* __restri
     if (tid == 0) bound_s = (int)b;
   }
   __syncthreads();
-  const uint32_t bound = (uint32_t)bound_s << 16;
-
-  // candidates: key > cut_key, or key == cut_key at an index up to cut_index
-  uint32_t cut_key = bound;
-  int cut_index = 0x7fffffff;
-  float below = -INFINITY;               // largest logit that is no candidate
-  auto gather = [&]() {
+  // an element reaches the bound unless it is less: NaN does, and without a bound all do
+  const uint32_t bound_key = (uint32_t)bound_s << 16;
+  const float bound = bound_key ? key_value(bound_key) : -INFINITY;
+  const float base = exp_base(bound, es);
+  float s = 0.f;
+  // one bit per logit of a thread that reaches the bound, listed after the pass: no branch in it
+  uint64_t reach = 0;
+  int bit = 0, first = tid;              // the next piece's bit, and the piece of bit 0
+  auto list = [&]() {
+    if (reach) {
+      int p = atomicAdd(&count, __popcll(reach));
+      for (; reach; reach &= reach - 1, ++p) {
+        const int b = __builtin_ctzll(reach);
+        if (p < TOPK_CAND) at_s[p] = (first + b / VEC * NT) * VEC + b % VEC;
+      }
+    }
+  };
+  r.each([&](int at, auto& v) {
+    constexpr int N = count_of<decltype(v)>;
+    if constexpr (N > 1) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = N - 1; j >= 0; --j) {
+        const bool under = v[j] < bound;
+        s += under ? exp_near(v[j], es, base) : 0.f;
+        m = m << 1 | (under ? 0 : 1);
+      }
+      if (bit == 0) first = at / VEC;
+      reach |= (uint64_t)m << bit;
+      bit += N;
+      if (bit == CHUNK * VEC) {
+        list();
+        bit = 0;
+        reach = 0;
+      }
+    } else {
+      list();                            // what the pieces left, then the element behind them
+      reach = 0;
+      if (v[0] < bound) {
+        s += exp_near(v[0], es, base);
+      } else {
+        const int p = atomicAdd(&count, 1);
+        if (p < TOPK_CAND) at_s[p] = at;
+      }
+    }
+  });
+  list();
+  // log of the sum of exp(x / T) over the elements under the bound
+  const double sum = block_reduce<NT>((double)s, redd, SumOp());
+  int m = count;
+  const bool flood = m > TOPK_CAND;      // uniform over the workgroup, as all that follows from it
+  double log_under = sum > 0.0 ? (log2(sum) - drift_near(bound, es, base)) * 0.6931471805599453 + (double)bound * inv_t : -INFINITY;
+  if (flood || !(sum > 1e-20 && sum < 1e30)) {
+    // the exact cut: an element is taken up if key > cut_key, or key == cut_key at an index up to cut_index
+    uint32_t cut_key = bound_key;
+    int cut_index = 0x7fffffff;
+    if (flood) {
+      // the k-th largest logit's key, and how many of its equals belong to the k
+      auto count_over = [&](auto&& test) {
+        uint32_t c = 0;
+        r.each([&](int at, auto& v) {
+#pragma unroll
+          for (int j = 0; j < count_of<decltype(v)>; ++j) c += test(order_key(v[j]), at, j);
+        });
+        return (int64_t)block_reduce<NT>(c, redu, SumOp());
+      };
+      uint32_t kth = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = kth | 1u << bit;
+        if (count_over([&](uint32_t key, int, int) { return key >= trial; }) >= k) kth = trial;
+      }
+      const int64_t equals = k - count_over([&](uint32_t key, int, int) { return key > kth; });
+      int before = -1;                   // largest index that fewer than `equals` of them come up to
+      for (int bit = 30; bit >= 0; --bit) {
+        const int trial = before + (1 << bit);
+        if (count_over([&](uint32_t key, int at, int j) { return key == kth && at <= trial - j; }) < equals) before = trial;
+      }
+      cut_key = kth;
+      cut_index = before + 1;
+      __syncthreads();
+      if (tid == 0) count = 0;
+      __syncthreads();
+    }
+    float below = -INFINITY;             // largest logit that is not taken up
     r.each([&](int at, auto& v) {
 #pragma unroll
       for (int j = 0; j < count_of<decltype(v)>; ++j) {
         const uint32_t key = order_key(v[j]);
-        if (key > cut_key || (key == cut_key && at <= cut_index - j)) {
-          const int p = atomicAdd(&count, 1);
-          if (p < TOPK_CAND) cand[p] = full_key(key, at + j);
-        } else {
-          below = fmaxf(below, v[j]);
-        }
+        if (!(key > cut_key || (key == cut_key && at <= cut_index - j))) below = fmaxf(below, v[j]);
+        else if (flood) at_s[atomicAdd(&count, 1)] = at + j;                      // exactly k of them
       }
     });
-    __syncthreads();
-  };
-  gather();
-  int m = count;
-  if (m > TOPK_CAND) {                   // uniform over the workgroup
-    // the k-th largest logit's key, and how many of its equals belong to the k
-    auto count_over = [&](auto&& test) {
-      uint32_t c = 0;
-      r.each([&](int at, auto& v) {
+    below = block_reduce<NT>(below, redf, MaxOp());
+    const float ref = below == -INFINITY ? 0.f : below, b2 = exp_base(ref, es);
+    float s2 = 0.f;
+    r.each([&](int at, auto& v) {
 #pragma unroll
-        for (int j = 0; j < count_of<decltype(v)>; ++j) c += test(order_key(v[j]), at, j);
-      });
-      return (int64_t)block_reduce<NT>(c, redu, SumOp());
-    };
-    uint32_t kth = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t trial = kth | 1u << bit;
-      if (count_over([&](uint32_t key, int, int) { return key >= trial; }) >= k) kth = trial;
-    }
-    const int64_t equals = k - count_over([&](uint32_t key, int, int) { return key > kth; });
-    int before = -1;                     // largest index that fewer than `equals` of them come up to
-    for (int bit = 30; bit >= 0; --bit) {
-      const int trial = before + (1 << bit);
-      if (trial < 0) continue;
-      if (count_over([&](uint32_t key, int at, int j) { return key == kth && at <= trial - j; }) < equals) before = trial;
-    }
-    cut_key = kth;
-    cut_index = before + 1;
-    below = -INFINITY;
-    __syncthreads();
-    if (tid == 0) count = 0;
-    __syncthreads();
-    gather();                            // exactly k of them
-    m = k;
+      for (int j = 0; j < count_of<decltype(v)>; ++j) {
+        const uint32_t key = order_key(v[j]);
+        const bool taken = key > cut_key || (key == cut_key && at <= cut_index - j);
+        s2 += taken ? 0.f : exp_at(v[j], es, b2);
+      }
+    });
+    const double sum2 = block_reduce<NT>((double)s2, redd, SumOp());
+    log_under = (log2(sum2) - drift(ref, es, b2)) * 0.6931471805599453 + (double)ref * inv_t;   // log 0 = -inf
+    if (flood) m = k;
   }
 
-  float top_left = -INFINITY;            // largest logit among the candidates that are not taken
   for (int i = tid; i < m; i += NT) {
-    const uint64_t mine = cand[i];
+    const int at = at_s[i];
+    uint32_t u;
+    if constexpr (DT == BCFFT_F32) u = ((const uint32_t*)row)[at];
+    else u = ((const uint16_t*)row)[at];
+    raw[i] = u;
+    cand[i] = full_key(order_key(DT == BCFFT_F32 ? __uint_as_float(u) : unpack16<DT == BCFFT_F32 ? BCFFT_BF16 : DT>(u).x), at);
+  }
+  __syncthreads();
+  for (int i = tid; i < m; i += NT) {
+    const uint64_t key = cand[i];
     int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < m; ++j) rank += cand[j] > mine;
-    const uint32_t at = ~(uint32_t)mine;
+#pragma unroll 8
+    for (int j = 0; j < m; ++j) rank += cand[j] > key;
     if (rank < k) {
-      if constexpr (DT == BCFFT_F32) ((uint32_t*)values)[n * k + rank] = ((const uint32_t*)row)[at];
-      else ((uint16_t*)values)[n * k + rank] = ((const uint16_t*)row)[at];
-      indices[n * k + rank] = (int32_t)at;
+      if constexpr (DT == BCFFT_F32) ((uint32_t*)values)[n * k + rank] = raw[i];
+      else ((uint16_t*)values)[n * k + rank] = (uint16_t)raw[i];
+      indices[n * k + rank] = (int32_t)~(uint32_t)key;
     } else {
-      const float v = key_value((uint32_t)(mine >> 32));
-      left[rank] = v;
-      top_left = fmaxf(top_left, v);
+      left[rank] = key_value((uint32_t)(key >> 32));
     }
   }
-  const float mr = block_reduce<NT>(fmaxf(below, top_left), redf, MaxOp());
-  const float ref = mr == -INFINITY ? 0.f : mr;
-  float s = 0.f;
-  r.each([&](int at, auto& v) {
-#pragma unroll
-    for (int j = 0; j < count_of<decltype(v)>; ++j) {
-      const uint32_t key = order_key(v[j]);
-      const bool taken = key > cut_key || (key == cut_key && at <= cut_index - j);
-      s += taken ? 0.f : exp_scaled(v[j] - ref, es);
+  if (m > k) __syncthreads();            // candidates that were not taken join the rest, in rank order
+  if (tid < 64) {
+    double log_left = -INFINITY;
+    if (m > k) {
+      const double top = (double)left[k] * inv_t;
+      double e = 0.0;
+      if (top == INFINITY) {
+        log_left = top;
+      } else if (!(top == -INFINITY)) {
+        for (int i = k + tid; i < m; i += 64) e += exp((double)left[i] * inv_t - top);
+        e = wave_reduce(e, SumOp());
+        log_left = top + log(e);
+      }
     }
-  });
-  for (int i = k + tid; i < m; i += NT) s += exp_scaled(left[i] - ref, es);
-  const double sum = block_reduce<NT>((double)s, redd, SumOp());
-  if (tid == 0) rest[n] = (float)((double)ref * inv_t + log(sum));      // log 0 = -inf: nothing left
+    if (tid == 0) {
+      const double hi = log_left > log_under || log_left != log_left ? log_left : log_under;
+      const double lo = log_left > log_under || log_left != log_left ? log_under : log_left;
+      rest[n] = (float)(lo == -INFINITY ? hi : hi + log1p(exp(lo - hi)));
+    }
+  }
 }
 
 // ------------------------------------------------------------------ the student's loss and gradient
@@ -328,24 +413,34 @@ struct DistillArgs {
 
 // LDS of a row's entries, behind them the bitmap of the vocabulary
 struct Entries {
-  double p[TOPK_MAX];                    // teacher's logit over T, then its probability
+  double p[TOPK_MAX];                    // teacher's logit over T, then exp(that - the largest)
   float s[TOPK_MAX];                     // student's logit
   int32_t at[TOPK_MAX];                  // index, or -1
-  double redd[16];
+  double redd[4][16];
+  double topd[16];
   float redf[16];
   int dup;
 };
 
-// Loads the entries, sets the bitmap, computes the teacher's softmax: p[j] = exp(a_j - am) and their
-// sum; false where the row has no mass to learn from. `am` and `total` come back in every thread.
+// the bits of elements `at` .. `at + N` of one piece; bytes, as a piece of 8 is one
+template <int N>
+__device__ __forceinline__ uint32_t piece_bits(const uint32_t* bits, int at) {
+  const uint32_t b = ((const uint8_t*)bits)[at >> 3];
+  return N == 8 ? b : b >> (at & 7) & ((1u << N) - 1);
+}
+// e, or 0 where bit j of a piece is set: two operations
+__device__ __forceinline__ float unless(uint32_t not_bits, int j, float e) {
+  return __uint_as_float(__float_as_uint(e) & (uint32_t)__builtin_amdgcn_sbfe((int)not_bits, (uint32_t)j, 1u));
+}
+
+// Loads the entries and sets the bitmap; the largest teacher logit over T of this thread's entries
 template <int DT, int NT>
-__device__ __forceinline__ bool teacher_softmax(const DistillArgs& a, int64_t n, const char* row, Entries& en,
-                                                uint32_t* bits, double& am, double& total, double& rest_p) {
+__device__ __forceinline__ double load_entries(const DistillArgs& a, int64_t n, const char* row, Entries& en, uint32_t* bits) {
   const int tid = threadIdx.x;
-  for (int64_t w = tid; w < (a.vocab + 31) / 32; w += NT) bits[w] = 0;
+  for (int w = tid; w < (int)((a.vocab + 31) / 32); w += NT) bits[w] = 0;
   if (tid == 0) en.dup = 0;
   __syncthreads();
-  double mx = -INFINITY;
+  double mx = a.rest && tid == 0 ? (double)a.rest[n] : -INFINITY;
   for (int j = tid; j < a.k; j += NT) {
     const int64_t e = n * a.k + j;
     const int64_t at = a.idx64 ? ((const int64_t*)a.indices)[e] : (int64_t)((const int32_t*)a.indices)[e];
@@ -357,24 +452,10 @@ __device__ __forceinline__ bool teacher_softmax(const DistillArgs& a, int64_t n,
     if (ok && (atomicOr(&bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1)) en.dup = 1;
     mx = t > mx || t != t ? t : mx;      // NaN stays: it makes the row NaN, as in a softmax
   }
-  const double rest = a.rest ? (double)a.rest[n] : -INFINITY;
-  mx = rest > mx || rest != rest ? rest : mx;
-  mx = block_reduce<NT>(mx, en.redd, MaxOp());
-  am = mx;
-  if (mx == -INFINITY) return false;     // (a NaN among the terms below makes the sum NaN)
-  double sum = 0.0;
-  for (int j = tid; j < a.k; j += NT) {
-    const double p = en.at[j] >= 0 ? exp(en.p[j] - mx) : 0.0;
-    sum += p;
-  }
-  rest_p = a.rest ? exp(rest - mx) : 0.0;
-  total = block_reduce<NT>(sum, en.redd, SumOp()) + rest_p;
-  rest_p /= total;
-  return true;
+  return mx;
 }
 
-// 1 where entry j is the first with its index; mass: the probability of all entries with that index
-template <int NT>
+// whether entry j is the first with its index; mass: the sum of p over all entries with that index
 __device__ __forceinline__ bool first_of(const Entries& en, int k, int j, double& mass) {
   if (!en.dup) return true;
   const int at = en.at[j];
@@ -411,41 +492,36 @@ __device__ __forceinline__ void store_piece(void* row, int64_t at, const float (
   }
 }
 
-// the bits of elements `at` .. `at + N` of one piece
-template <int N>
-__device__ __forceinline__ uint32_t piece_bits(const uint32_t* bits, int at) {
-  return bits[at >> 5] >> (at & 31) & ((1u << N) - 1);
-}
-
-// The whole gradient row: elements outside the entries are exp(x / T) times `coef` (0 where the entry
-// sits, written after), then the entries. The wait makes the pieces' stores complete (acknowledged by
-// L2) before other waves of the workgroup store the entries into the same lines.
-template <int DT, int NT, class ROW>
-__device__ __forceinline__ void write_gradient(const DistillArgs& a, int64_t n, ROW& r, Entries& en,
-                                               const uint32_t* bits, float ref, float coef, float m_all,
-                                               float inv_s, double total, float scale) {
-  constexpr int E = DT == BCFFT_F32 ? 4 : 2;
-  char* out = (char*)a.grad + n * a.vocab * E;
-  const float c = coef * scale;
-  r.each([&](int at, auto& v) {
-    constexpr int N = count_of<decltype(v)>;
-    const uint32_t b = piece_bits<N>(bits, at);
-    float g[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) g[j] = b >> j & 1 ? 0.f : exp_scaled(v[j] - ref, a.es) * c;
-    store_piece<DT>(out, at, g);
-  });
+// The entries' gradients, over the zeros that the pass before them left there. The wait makes that pass's
+// stores complete (acknowledged by L2) before other waves of the workgroup store into the same lines.
+template <int DT, int NT>
+__device__ __forceinline__ void write_entries(const DistillArgs& a, int64_t n, Entries& en, float m_all, double inv_s,
+                                              double inv_total, float scale) {
+  char* out = (char*)a.grad + n * a.vocab * (DT == BCFFT_F32 ? 4 : 2);
   wait_vmcnt<0>();
   __syncthreads();
   for (int j = threadIdx.x; j < a.k; j += NT) {
     if (en.at[j] < 0) continue;
     double mass = en.p[j];
-    if (!first_of<NT>(en, a.k, j, mass)) continue;
-    const float q = exp_scaled(en.s[j] - m_all, a.es) * inv_s;
-    store_one<DT>(out, en.at[j], (q - (float)(mass / total)) * scale);
+    if (!first_of(en, a.k, j, mass)) continue;
+    const double q = exp(((double)en.s[j] - (double)m_all) * a.inv_t) * inv_s;
+    store_one<DT>(out, en.at[j], (float)(q - mass * inv_total) * scale);
   }
 }
-
+// The other elements': exp((v - ref) / T) times coef
+template <int DT, class ROW>
+__device__ __forceinline__ void write_others(const DistillArgs& a, int64_t n, ROW& r, const uint32_t* bits, float base,
+                                             float coef) {
+  char* out = (char*)a.grad + n * a.vocab * (DT == BCFFT_F32 ? 4 : 2);
+  r.each([&](int at, auto& v) {
+    constexpr int N = count_of<decltype(v)>;
+    const uint32_t keep = ~piece_bits<N>(bits, at);
+    float g[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] = unless(keep, j, exp_at(v[j], a.es, base) * coef);
+    store_piece<DT>(out, at, g);
+  });
+}
 template <int DT, int NT>
 __device__ __forceinline__ void write_zero(const DistillArgs& a, int64_t n) {
   constexpr int VEC = RowType<DT>::VEC;
@@ -457,27 +533,46 @@ __device__ __forceinline__ void write_zero(const DistillArgs& a, int64_t n) {
   if (end < a.vocab) store_one<DT>(out, end, 0.f);
 }
 
-// Loss of a row and, with GRAD, its gradient, in one read of the row. The sums are kept apart: the
-// entries' relative to their largest logit, the others' relative to theirs, so that neither underflows
-// whatever lies between them.
+// Loss of a row and, with GRAD, its gradient, in one read of the row.
+// 1. the row's maximum                                                             1.5 operations a logit
+// 2. the sum of the exponentials outside the entries, the entries' own in fp64 beside it               10
+// 3. gradient: the exponentials from 2, where up to 64 per thread stay in registers                   1.5
+// Where the sum of 2 vanishes in fp32 (all of the row 45 T below its maximum but the entries) and the
+// teacher's rest needs its logarithm, 2 runs again relative to the others' own maximum.
 template <int DT, int NT, int HOLD, bool GRAD>
-__global__ __launch_bounds__(NT) void bc_distill_kernel(DistillArgs a) {
-  constexpr int E = DT == BCFFT_F32 ? 4 : 2;
+__global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill_kernel(DistillArgs a) {
+  constexpr int E = DT == BCFFT_F32 ? 4 : 2, VEC = RowType<DT>::VEC;
+  constexpr bool KEEP = GRAD && HOLD > 0 && HOLD * VEC <= 64;
   __shared__ Entries en;
   extern __shared__ uint32_t bits[];
-  using ROW = Row<DT, NT, HOLD>;
   const int tid = threadIdx.x;
   const int64_t n = blockIdx.x;
   const float w = a.weight ? a.weight[n] : 1.f;
   const char* row = (const char*)a.logits + n * a.row_stride * E;
-  double am = 0.0, total = 1.0, rest_p = 0.0;
-  ROW r;
-  bool live = w != 0.f;                  // uniform: a row of weight 0 is not read
-  if (live) {
+  Row<DT, NT, HOLD> r;
+  double am = -INFINITY;
+  if (w != 0.f) {                        // uniform: a row of weight 0 is not read
     r.open(row, a.vocab);
-    live = teacher_softmax<DT, NT>(a, n, row, en, bits, am, total, rest_p);
+    am = load_entries<DT, NT>(a, n, row, en, bits);
   }
-  if (!live) {
+  float mx = -INFINITY;
+  if (w != 0.f) {
+    r.each([&](int, auto& v) {
+#pragma unroll
+      for (int j = 0; j + 1 < count_of<decltype(v)>; j += 2) mx = fmaxf(fmaxf(mx, v[j]), v[j + 1]);
+      if constexpr (count_of<decltype(v)> == 1) mx = fmaxf(mx, v[0]);
+    });
+  }
+  am = wave_reduce(am, MaxOp());
+  mx = wave_reduce(mx, MaxOp());
+  if ((tid & 63) == 0) {
+    en.topd[tid >> 6] = am;
+    en.redf[tid >> 6] = mx;
+  }
+  __syncthreads();
+  am = across_waves<NT>(en.topd, MaxOp());
+  mx = across_waves<NT>(en.redf, MaxOp());
+  if (am == -INFINITY) {                 // no teacher mass (or weight 0): uniform over the workgroup
     if (tid == 0) {
       a.loss[n] = 0.f;
       if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * n) = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -485,60 +580,137 @@ __global__ __launch_bounds__(NT) void bc_distill_kernel(DistillArgs a) {
     if constexpr (GRAD) write_zero<DT, NT>(a, n);
     return;
   }
-  // maxima of the two parts
-  float mo = -INFINITY, me = -INFINITY;
-  r.each([&](int at, auto& v) {
-    constexpr int N = count_of<decltype(v)>;
-    const uint32_t b = piece_bits<N>(bits, at);
-#pragma unroll
-    for (int j = 0; j < N; ++j) mo = fmaxf(mo, b >> j & 1 ? -INFINITY : v[j]);
-  });
-  for (int j = tid; j < a.k; j += NT) me = fmaxf(me, en.s[j]);
-  mo = block_reduce<NT>(mo, en.redf, MaxOp());
-  me = block_reduce<NT>(me, en.redf, MaxOp());
-  const float ro = mo == -INFINITY ? 0.f : mo, re = me == -INFINITY ? 0.f : me;
-  // their sums, and the loss's part that is linear in the logits
-  float so = 0.f;
-  r.each([&](int at, auto& v) {
-    constexpr int N = count_of<decltype(v)>;
-    const uint32_t b = piece_bits<N>(bits, at);
-#pragma unroll
-    for (int j = 0; j < N; ++j) so += b >> j & 1 ? 0.f : exp_scaled(v[j] - ro, a.es);
-  });
-  double se = 0.0, lin = 0.0;
+  const float m_all = mx == -INFINITY ? 0.f : mx, base = exp_base(m_all, a.es);
+
+  // sums over the entries: the teacher's total, the student's, the loss's part linear in the logits. Before
+  // the pass over the row: fp64 functions take 40 registers
+  double total = 0.0, se = 0.0, lin = 0.0;
   for (int j = tid; j < a.k; j += NT) {
     if (en.at[j] < 0) continue;
-    const double t = en.p[j] - am, p = exp(t), x = ((double)en.s[j] - (double)re) * a.inv_t;
-    en.p[j] = p;                         // (read again by first_of, after a barrier)
+    const double t = en.p[j] - am, p = exp(t), x = ((double)en.s[j] - (double)m_all) * a.inv_t;
+    en.p[j] = p;
+    total += p;
     if (p > 0.0) lin += p * (t - x);
     else if (p != p) lin = p;
+    if (!en.dup) se += exp(x);
   }
-  const double sum_o = block_reduce<NT>((double)so, en.redd, SumOp());
-  for (int j = tid; j < a.k; j += NT) {
-    double mass;
-    if (en.at[j] >= 0 && first_of<NT>(en, a.k, j, mass)) se += exp(((double)en.s[j] - (double)re) * a.inv_t);
+  if (en.dup) {                          // uniform: each index once
+    __syncthreads();
+    for (int j = tid; j < a.k; j += NT) {
+      double mass;
+      if (en.at[j] >= 0 && first_of(en, a.k, j, mass)) se += exp(((double)en.s[j] - (double)m_all) * a.inv_t);
+    }
   }
-  const double sum_e = block_reduce<NT>(se, en.redd, SumOp());
-  lin = block_reduce<NT>(lin, en.redd, SumOp()) / total;
-  const float m_top = fmaxf(mo, me), m_all = m_top == -INFINITY ? 0.f : m_top;
-  const double fo = mo == -INFINITY ? 0.0 : (double)exp_scaled(mo - m_all, a.es);
-  const double fe = me == -INFINITY ? 0.0 : (double)exp_scaled(me - m_all, a.es);
-  const double sum = sum_o * fo + sum_e * fe;
-  const float inv_s = (float)(1.0 / sum);
-  const float coef = (float)(fo / sum - (rest_p != 0.0 && sum_o != 0.0 ? rest_p / sum_o : 0.0));
+  // the other elements' sum
+  float so = 0.f;
+  float kept[KEEP ? HOLD : 1][VEC], kept_tail = 0.f;
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      const int p = i * NT + tid;
+      if (p < (int)r.pieces) {
+        float v[VEC];
+        unpack<DT>(r.held[i], v);
+        const uint32_t keep = ~piece_bits<VEC>(bits, p * VEC);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          kept[i][j] = unless(keep, j, exp_at(v[j], a.es, base));
+          so += kept[i][j];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (tid < r.tail) {
+      kept_tail = unless(~piece_bits<1>(bits, (int)(r.pieces * VEC) + tid), 0, exp_at(r.last, a.es, base));
+      so += kept_tail;
+    }
+  } else {
+    r.each([&](int at, auto& v) {
+      constexpr int N = count_of<decltype(v)>;
+      const uint32_t keep = ~piece_bits<N>(bits, at);
+#pragma unroll
+      for (int j = 0; j < N; ++j) so += unless(keep, j, exp_at(v[j], a.es, base));
+    });
+  }
+  double sums[4] = {(double)so, total, se, lin};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sums[q] = wave_reduce(sums[q], SumOp());
+  if ((tid & 63) == 0) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) en.redd[q][tid >> 6] = sums[q];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sums[q] = across_waves<NT>(en.redd[q], SumOp());
+  const double rest_a = a.rest ? (double)a.rest[n] - am : -INFINITY, rest_e = exp(rest_a);
+  const double inv_total = 1.0 / (sums[1] + rest_e), rest_p = rest_e * inv_total;
+  double sum_o = sums[0] * exp2(-drift(m_all, a.es, base));      // relative to m_all
+  const double sum_e = sums[2];
+  float ref = m_all;
+  double sum_ref = sum_o;                // the others' sum relative to ref
+  const bool again = rest_p != 0.0 && sum_o < 1e-20;             // uniform
+  if (again) {
+    float mo = -INFINITY;
+    Row<DT, NT, 0> r2;
+    r2.open(row, a.vocab);
+    r2.each([&](int at, auto& v) {
+      constexpr int N = count_of<decltype(v)>;
+      const uint32_t b = piece_bits<N>(bits, at);
+#pragma unroll
+      for (int j = 0; j < N; ++j) mo = fmaxf(mo, b >> j & 1 ? -INFINITY : v[j]);
+    });
+    mo = block_reduce<NT>(mo, en.redf, MaxOp());
+    ref = mo == -INFINITY ? 0.f : mo;
+    const float b2 = exp_base(ref, a.es);
+    float s2 = 0.f;
+    r2.each([&](int at, auto& v) {
+      constexpr int N = count_of<decltype(v)>;
+      const uint32_t keep = ~piece_bits<N>(bits, at);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s2 += unless(keep, j, exp_at(v[j], a.es, b2));
+    });
+    sum_ref = block_reduce<NT>((double)s2, en.topd, SumOp()) * exp2(-drift(ref, a.es, b2));
+    sum_o = mo == -INFINITY ? 0.0 : sum_ref * exp(((double)ref - (double)m_all) * a.inv_t);
+  }
+  const double sum = sum_o + sum_e, inv_s = 1.0 / sum;
+  // d loss / d s of an element outside the entries, over exp((v - ref) / T)
+  const double shift = ref == m_all ? 1.0 : exp(((double)ref - (double)m_all) * a.inv_t);
+  const double coef = shift * inv_s - (rest_p != 0.0 && sum_ref != 0.0 ? rest_p / sum_ref : 0.0);
   if (tid == 0) {
-    // lin holds sum_j P_j ((a_j - am) - (s_j - re) / T); the logarithms of both sums and the shift of
-    // the student's reference from re to m_all complete it
-    const double ls = log((mo == -INFINITY ? 0.0 : sum_o * exp(((double)mo - (double)m_all) * a.inv_t)) +
-                          (me == -INFINITY ? 0.0 : sum_e * exp(((double)me - (double)m_all) * a.inv_t)));
-    const double shift = ((double)re - (double)m_all) * a.inv_t;
-    double loss = lin - (1.0 - rest_p) * shift + ls - log(total);
-    if (rest_p != 0.0)
-      loss += rest_p * (((double)a.rest[n] - am) - (((double)ro - (double)m_all) * a.inv_t + log(sum_o)));
+    // sum_j P_j ((a_j - am) - (s_j - m_all) / T) + log sum - log total, and the rest's part
+    double loss = sums[3] * inv_total + log(sum) + log(inv_total);
+    if (rest_p != 0.0) loss += rest_p * (rest_a - (((double)ref - (double)m_all) * a.inv_t + log(sum_ref)));
     a.loss[n] = (float)loss * w;
-    if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * n) = make_float4(ro, coef, m_all, inv_s);
+    if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * n) = make_float4(ref, (float)coef, m_all, (float)inv_s);
   }
-  if constexpr (GRAD) write_gradient<DT, NT>(a, n, r, en, bits, ro, coef, m_all, inv_s, total, (float)(w * a.inv_t));
+  if constexpr (GRAD) {
+    const float scale = (float)(w * a.inv_t);
+    if (KEEP && !again) {
+      char* out = (char*)a.grad + n * a.vocab * E;
+      const float c = (float)(coef * exp2(-drift(m_all, a.es, base))) * scale;
+#pragma unroll
+      for (int i = 0; i < (KEEP ? HOLD : 0); ++i) {
+        const int p = i * NT + tid;
+        if (p < (int)r.pieces) {
+          float g[VEC];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) g[j] = kept[i][j] * c;
+          store_piece<DT>(out, p * VEC, g);
+        }
+      }
+      if (tid < r.tail) store_one<DT>(out, r.pieces * VEC + tid, kept_tail * c);
+    } else {
+      const float b = exp_base(ref, a.es), c = (float)(coef * exp2(-drift(ref, a.es, b))) * scale;
+      if (HOLD > 0 && !KEEP) {
+        write_others<DT>(a, n, r, bits, b, c);
+      } else {
+        Row<DT, NT, 0> r2;
+        r2.open(row, a.vocab);
+        write_others<DT>(a, n, r2, bits, b, c);
+      }
+    }
+    write_entries<DT, NT>(a, n, en, m_all, inv_s, inv_total, scale);
+  }
 }
 
 // Gradient from the forward's sums: one read of the row, one write
@@ -547,21 +719,28 @@ __global__ __launch_bounds__(NT) void bc_distill_backward_kernel(DistillArgs a) 
   constexpr int E = DT == BCFFT_F32 ? 4 : 2;
   __shared__ Entries en;
   extern __shared__ uint32_t bits[];
-  using ROW = Row<DT, NT, 0>;
   const int64_t n = blockIdx.x;
   const float w = a.weight ? a.weight[n] : 1.f;
   const char* row = (const char*)a.logits + n * a.row_stride * E;
-  double am = 0.0, total = 1.0, rest_p = 0.0;
-  if (w == 0.f || !teacher_softmax<DT, NT>(a, n, row, en, bits, am, total, rest_p)) {
+  double am = -INFINITY;
+  if (w != 0.f) am = block_reduce<NT>(load_entries<DT, NT>(a, n, row, en, bits), en.topd, MaxOp());   // uniform
+  if (am == -INFINITY) {
     write_zero<DT, NT>(a, n);
     return;
   }
-  for (int j = threadIdx.x; j < a.k; j += NT)
-    if (en.at[j] >= 0) en.p[j] = exp(en.p[j] - am);
+  double total = 0.0;
+  for (int j = threadIdx.x; j < a.k; j += NT) {
+    if (en.at[j] < 0) continue;
+    en.p[j] = exp(en.p[j] - am);
+    total += en.p[j];
+  }
+  total = block_reduce<NT>(total, en.topd, SumOp()) + (a.rest ? exp((double)a.rest[n] - am) : 0.0);
   const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * n);
-  ROW r;
+  const float scale = (float)(w * a.inv_t) * a.upstream[n], base = exp_base(st.x, a.es);
+  Row<DT, NT, 0> r;
   r.open(row, a.vocab);
-  write_gradient<DT, NT>(a, n, r, en, bits, st.x, st.y, st.z, st.w, total, (float)(w * a.inv_t) * a.upstream[n]);
+  write_others<DT>(a, n, r, bits, base, st.y * (float)exp2(-drift(st.x, a.es, base)) * scale);
+  write_entries<DT, NT>(a, n, en, st.z, st.w, 1.0 / total, scale);
 }
 
 // ------------------------------------------------------------------ launches
