@@ -31,7 +31,7 @@ struct DzArgs {
   int64_t ldz;
   float* part;                           // column sums per slice of rows, or null
   int64_t m, n;
-  int act;
+  int act, rows;                         // rows per workgroup (dz)
 };
 
 // how a product is cut: tile kind (0: few rows, 1: 128 x 128, 2: 256 x 128, 3: 256 x 256) and slices of k
@@ -119,12 +119,31 @@ __device__ __forceinline__ void store4_at(void* p, int64_t i, int cnt, const flo
 }
 
 // ------------------------------------------------------------------ activations (fp32)
-// gelu is z times the normal distribution function, 0.5 erfc(-z / sqrt 2): no cancellation for z < 0
+// The normal distribution function Phi(z) = erfc(-z / sqrt 2) / 2: for x = |z| / sqrt 2 and t = 1 / (1 + 0.45 x),
+// erfc(x) = t exp(-x^2 + p(t)), p the degree 9 Chebyshev fit to log(erfcx(x) / t) over x in [0, 10] (fit error
+// 1.3e-8; in fp32 within 2.3e-7 of Phi, 5e-6 relative down to z = -6). A third of the instructions of the
+// library's erfc: with that one the epilogue of 2048 x 4096 outputs took half as long as their product.
+__device__ __forceinline__ float normal_cdf(float z) {
+  const float x = fabsf(z) * 0.70710678f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.45f, x, 1.f));
+  float p = 0.183369572f;
+  p = fmaf(p, t, -1.043303666f);
+  p = fmaf(p, t, 2.375441185f);
+  p = fmaf(p, t, -2.667089331f);
+  p = fmaf(p, t, 1.544028557f);
+  p = fmaf(p, t, -0.7029624839f);
+  p = fmaf(p, t, 0.3095381628f);
+  p = fmaf(p, t, 0.3691916272f);
+  p = fmaf(p, t, 1.002771143f);
+  p = fmaf(p, t, -1.370984761f);
+  const float q = 0.5f * t * __expf(fmaf(-x, x, p));
+  return z < 0.f ? q : 1.f - q;
+}
 __device__ __forceinline__ float act_value(int act, float z) {
   switch (act) {
     case BCFFT_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
     case BCFFT_ACT_SILU: return silu(z);
-    case BCFFT_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);
+    case BCFFT_ACT_GELU: return z * normal_cdf(z);
     default: return z;
   }
 }
@@ -142,7 +161,7 @@ __device__ __forceinline__ void act_both(int act, float z, float& v, float& slop
       break;
     }
     case BCFFT_ACT_GELU: {
-      const float phi = 0.5f * erfcf(-0.70710678f * z);
+      const float phi = normal_cdf(z);
       v = z * phi;
       slope = phi + z * 0.39894228f * __expf(-0.5f * z * z);
       break;

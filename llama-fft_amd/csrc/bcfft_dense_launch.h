@@ -3,6 +3,8 @@
 #pragma once
 #include "bcfft_dense_tile.h"
 
+#include <atomic>
+
 namespace bcfft {
 
 // sums the slices of a split k in order and finishes the output
@@ -110,7 +112,14 @@ static void launch_tile(const DenseArgs& a, hipStream_t s) {
   constexpr int BR = GLU ? BN / 2 : BN;
   constexpr unsigned lds = (RA * BM + RB * BN) * 128;
   auto kern = bc_dense_tile_kernel<DT, CA, CB, BM, BN, WM, WN, RA, RB, GLU>;
-  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  // once per device: the attribute call costs the host as much as the launch
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  if (dev > 63 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
+    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (dev <= 63) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   const unsigned tiles = (unsigned)(((a.m + BM - 1) / BM) * ((a.n + BR - 1) / BR));
   hipLaunchKernelGGL(kern, dim3(tiles, (unsigned)a.kz), dim3(64 * WM * WN), lds, s, a);
 }
