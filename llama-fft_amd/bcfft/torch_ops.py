@@ -10,6 +10,8 @@ a host tensor fails loudly as in bcfft.ops.
     torch.ops.bcfft.spectra(c, transpose_conj) -> spec
     torch.ops.bcfft.forward_glu(x2d, spec_gu, block_size, gate_features, algo) -> h
     torch.ops.bcfft.forward_mlp(x2d, spec_gu, spec_down, block_size, inter_features, mode) -> y
+    torch.ops.bcfft.dense_linear(x, weight, bias, residual, activation) -> y (forward only)
+    torch.ops.bcfft.dense_glu(x, w_gate, w_up, activation) -> h (forward only)
     torch.ops.bcfft.topk_logits(logits, k, temperature) -> values, indices, rest
     torch.ops.bcfft.topk_kl(logits, values, indices, rest, weight, temperature) -> loss (forward only)
     torch.ops.bcfft.topk_kl_grad(...) -> loss, dlogits
@@ -18,7 +20,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib, distill, ops
+from . import _lib, dense, distill, ops
 
 
 @torch.library.custom_op("bcfft::forward", mutates_args=())
@@ -84,6 +86,36 @@ def _forward_mlp_fake(x2d, spec_gu, spec_down, block_size, inter_features, mode=
     return x2d.new_empty(x2d.shape)
 
 
+@torch.library.custom_op("bcfft::dense_linear", mutates_args=())
+def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                 residual: torch.Tensor | None = None, activation: str = "none") -> torch.Tensor:
+    """act(x W^T + bias) + residual: bcfft.dense.linear's forward (the projections that
+    patch_llama_fft.py:343-394 leaves dense)."""
+    with torch.no_grad():
+        return dense.linear(x, weight, bias, activation=None if activation == "none" else activation, residual=residual)
+
+
+@dense_linear.register_fake
+def _dense_linear_fake(x, weight, bias=None, residual=None, activation="none"):
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError("bcfft::dense_linear: weight must be (out_features, in_features)")
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
+@torch.library.custom_op("bcfft::dense_glu", mutates_args=())
+def dense_glu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """act(x Wg^T) * (x Wu^T): bcfft.dense.glu's forward (the dense MLP's inner product)."""
+    with torch.no_grad():
+        return dense.glu(x, w_gate, w_up, activation=None if activation == "none" else activation)
+
+
+@dense_glu.register_fake
+def _dense_glu_fake(x, w_gate, w_up, activation="silu"):
+    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape[1] != x.shape[-1] or w_up.shape != w_gate.shape:
+        raise ValueError("bcfft::dense_glu: w_gate and w_up must be (out_features, in_features)")
+    return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
+
+
 @torch.library.custom_op("bcfft::topk_logits", mutates_args=())
 def topk_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """A teacher's k largest logits, indices and rest: bcfft.distill.topk_logits (calibrate_bc.py:192-212)."""
@@ -129,8 +161,9 @@ def _topk_kl_grad_fake(logits, values, indices, rest=None, weight=None, temperat
 def registered() -> bool:
     """True once the ops are visible under torch.ops.bcfft (importing this module registers them)."""
     return all(hasattr(torch.ops.bcfft, n) for n in ("forward", "spectra", "forward_glu", "forward_mlp",
-                                                          "topk_logits", "topk_kl", "topk_kl_grad"))
+                                                          "topk_logits", "topk_kl", "topk_kl_grad", "dense_linear",
+                                                          "dense_glu"))
 
 
 __all__ = ["forward", "spectra", "forward_glu", "forward_mlp", "topk_logits", "topk_kl", "topk_kl_grad",
-           "registered", "_lib"]
+           "dense_linear", "dense_glu", "registered", "_lib"]

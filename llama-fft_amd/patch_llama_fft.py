@@ -28,6 +28,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
+from bcfft import dense as _dense
 from bcfft import ops as _ops
 from bcfft import _lib
 from fft_utils import circulant_matvec_fft
@@ -453,6 +454,46 @@ def fuse_mlp_gate_up(model) -> int:
             continue
         object.__setattr__(mlp, "_bc_gate_up", BCFusedGateUp(g, u))
         mlp.forward = types.MethodType(_fused_mlp_forward, mlp)
+        n += 1
+    return n
+
+
+def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
+    """The dense kernels take device tensors of one dtype; anything else runs the modules' own forward."""
+    ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
+    return (x.is_cuda and x.dtype in _lib.DTYPE_CODE and not torch.is_autocast_enabled("cuda")
+            and all(t is None or (t.dtype == x.dtype and t.device == x.device) for t in ws))
+
+
+def _dense_mlp_forward(self, x, residual=None):
+    """down(silu(gate(x)) * up(x)) (+ residual, in the down projection's epilogue) in two launches."""
+    if not _dense_mlp_ok(self, x):
+        y = self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+        return y if residual is None else y + residual
+    h = _dense.glu(x, self.gate_proj.weight, self.up_proj.weight, activation="silu")
+    return _dense.linear(h, self.down_proj.weight, self.down_proj.bias, residual=residual)
+
+
+def fuse_dense_mlp(model) -> int:
+    """Route the MLPs that a patch leaves dense (nn.Linear gate_proj / up_proj without bias, act = SiLU;
+    31 of 32 layers with the reference's default NUM_LAYERS_TO_PATCH) through the dense kernels: the gate and
+    up projections with their product in one launch, the down projection in another, in training too
+    (bcfft.dense is differentiable in every operand). The rewired forward also takes a residual that the
+    down projection adds in its epilogue. Parameters and state_dict are unchanged; replacing one of the
+    three modules afterwards needs a new call. Returns the number of MLPs rewired."""
+    import types
+    n = 0
+    for layer in model.model.layers:
+        mlp = getattr(layer, "mlp", None)
+        mods = [getattr(mlp, nm, None) for nm in MLP_PROJECTIONS] if mlp is not None else []
+        if len(mods) != 3 or not all(type(m) is nn.Linear for m in mods):
+            continue
+        act = getattr(mlp, "act_fn", None)          # nn.SiLU, or transformers' SiLUActivation
+        if mods[0].bias is not None or mods[1].bias is not None:
+            continue
+        if not (isinstance(act, nn.SiLU) or type(act).__name__ == "SiLUActivation"):
+            continue
+        mlp.forward = types.MethodType(_dense_mlp_forward, mlp)
         n += 1
     return n
 

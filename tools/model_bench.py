@@ -288,12 +288,16 @@ def main(argv=None):
             patch(model, num_layers_to_patch=n_patch, block_size=b, patch_position=args.patch_position)
         n_qkv = P.fuse_attention_qkv(model)
         n_glu = P.fuse_mlp_gate_up(model)
+        n_dense = P.fuse_dense_mlp(model)                       # the MLPs the patch leaves dense
         torch.cuda.synchronize()
         res["patch_s"] = time.perf_counter() - t0
         torch.cuda.empty_cache()
 
         student_last, t_bc = prefill(model, batches, args.warmup, args.runs)
         metrics = E.last_token_metrics(student_last, teacher_last, args.temperature, args.topk)
+        if teacher_last.is_cuda:                                # the calibration loss from the teacher's top logits
+            cache = E.teacher_cache(teacher_last, min(64, teacher_last.shape[-1]), args.temperature)
+            metrics["last_topk_kl"] = float(E.distill_kl(student_last, cache).mean())
         parity = projection_parity(model, patched[0], batches[0]) if patched else {}
         if args.new_tokens:
             res["bc_decode_s"] = decode(model, batches, args.new_tokens, cfg.pad_token_id)
@@ -326,6 +330,7 @@ def main(argv=None):
                            "prompts": args.prompts, "max_len": args.max_len,
                            "batch_size": args.batch_size, "tokens": total_tokens,
                            "fused_qkv_layers": n_qkv, "fused_gate_up_layers": n_glu,
+                           "fused_dense_mlp_layers": n_dense,
                            "parallelism": f"prompt-replicas x{world}"},
                 "prefill_ms": round(t_bc * 1e3, 3),
                 "dense_prefill_ms": round(t_dense * 1e3, 3),
