@@ -73,47 +73,68 @@ __device__ __forceinline__ uint4 load_part(const char* row, int64_t k, int64_t k
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// elements i .. i + cnt (cnt <= 4) of an array of DT as fp32, 0 past cnt
-template <int DT>
-__device__ __forceinline__ void load4_at(const void* p, int64_t i, int cnt, float (&v)[4]) {
-  if (cnt == 4) {
-    if constexpr (DT == BCFFT_F32) {
-      const Unaligned16<4> u = *reinterpret_cast<const Unaligned16<4>*>((const float*)p + i);
+// elements i .. i + cnt (cnt <= N, N = 1, 4 or 8) of an array of DT as fp32, 0 past cnt
+template <int DT, int N>
+__device__ __forceinline__ void load_at(const void* p, int64_t i, int cnt, float (&v)[N]) {
+  constexpr int E = DT == BCFFT_F32 ? 4 : 2;
+  if (N > 1 && cnt == N) {
+    uint32_t w[N * E / 4 > 0 ? N * E / 4 : 1];
+    if constexpr (N * E >= 16) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(u.w[j]);
-    } else {
-      const Unaligned8<2> u = *reinterpret_cast<const Unaligned8<2>*>((const uint16_t*)p + i);
-      const float2 a = unpack16<DT>(u.w[0]), b = unpack16<DT>(u.w[1]);
-      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+      for (int q = 0; q < N * E / 16; ++q) {
+        const Unaligned16<E> u = *reinterpret_cast<const Unaligned16<E>*>((const char*)p + i * E + 16 * q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[4 * q + j] = u.w[j];
+      }
+    } else if constexpr (N * E == 8) {
+      const Unaligned8<E> u = *reinterpret_cast<const Unaligned8<E>*>((const char*)p + i * E);
+      w[0] = u.w[0], w[1] = u.w[1];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (DT == BCFFT_F32) {
+        v[j] = __uint_as_float(w[j]);
+      } else if (j % 2 == 0) {
+        const float2 f = unpack16<DT>(w[j / 2]);
+        v[j] = f.x;
+        if (j + 1 < N) v[j + 1] = f.y;
+      }
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = j < cnt ? load_scalar(p, i + j, DT) : 0.f;
+    for (int j = 0; j < N; ++j) v[j] = j < cnt ? load_scalar(p, i + j, DT) : 0.f;
   }
 }
-template <int DT>
-__device__ __forceinline__ void store4_at(void* p, int64_t i, int cnt, const float (&v)[4]) {
-  if constexpr (DT == BCFFT_F32) {
-    if (cnt == 4) {
-      Unaligned16<4> u;
+template <int DT, int N>
+__device__ __forceinline__ void store_at(void* p, int64_t i, int cnt, const float (&v)[N]) {
+  constexpr int E = DT == BCFFT_F32 ? 4 : 2;
+  uint32_t w[(N * E + 3) / 4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u.w[j] = __float_as_uint(v[j]);
-      *reinterpret_cast<Unaligned16<4>*>((float*)p + i) = u;
-    } else {
+  for (int j = 0; j < N; ++j) {
+    if constexpr (DT == BCFFT_F32) w[j] = __float_as_uint(v[j]);
+    else if (j % 2 == 0) w[j / 2] = pack16<DT>(v[j], j + 1 < N ? v[j + 1] : 0.f);
+  }
+  if (N > 1 && cnt == N) {
+    if constexpr (N * E >= 16) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < cnt) ((float*)p)[i + j] = v[j];
+      for (int q = 0; q < N * E / 16; ++q) {
+        Unaligned16<E> u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u.w[j] = w[4 * q + j];
+        *reinterpret_cast<Unaligned16<E>*>((char*)p + i * E + 16 * q) = u;
+      }
+    } else if constexpr (N * E == 8) {
+      Unaligned8<E> u;
+      u.w[0] = w[0], u.w[1] = w[1];
+      *reinterpret_cast<Unaligned8<E>*>((char*)p + i * E) = u;
     }
   } else {
-    Unaligned8<2> u;
-    u.w[0] = pack16<DT>(v[0], v[1]);
-    u.w[1] = pack16<DT>(v[2], v[3]);
-    if (cnt == 4) {
-      *reinterpret_cast<Unaligned8<2>*>((uint16_t*)p + i) = u;
-    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < cnt) ((uint16_t*)p)[i + j] = (uint16_t)(u.w[j / 2] >> 16 * (j & 1));
+    for (int j = 0; j < N; ++j) {
+      if (j < cnt) {
+        if constexpr (DT == BCFFT_F32) ((uint32_t*)p)[i + j] = w[j];
+        else ((uint16_t*)p)[i + j] = (uint16_t)(w[j / 2] >> 16 * (j & 1));
+      }
     }
   }
 }
@@ -173,57 +194,56 @@ __device__ __forceinline__ void act_both(int act, float z, float& v, float& slop
 }
 
 // ------------------------------------------------------------------ output stages
-// four consecutive columns n .. n + cnt of row m, accumulated in fp32; one rounding
-template <int DT>
-__device__ __forceinline__ void finish_linear(const DenseArgs& a, int64_t m, int64_t n, f32x4 acc, int cnt) {
-  float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+// N consecutive columns n .. n + cnt of row m, accumulated in fp32; one rounding
+template <int DT, int N>
+__device__ __forceinline__ void finish_linear(const DenseArgs& a, int64_t m, int64_t n, float (&v)[N], int cnt) {
   if (a.bias) {
-    float b[4];
-    load4_at<DT>(a.bias, n, cnt, b);
+    float b[N];
+    load_at<DT>(a.bias, n, cnt, b);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += b[j];
+    for (int j = 0; j < N; ++j) v[j] += b[j];
   }
-  if (a.z) store4_at<BCFFT_F32>(a.z, m * a.n + n, cnt, v);
+  if (a.z) store_at<BCFFT_F32>(a.z, m * a.n + n, cnt, v);
   if (a.act != BCFFT_ACT_NONE) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = act_value(a.act, v[j]);
+    for (int j = 0; j < N; ++j) v[j] = act_value(a.act, v[j]);
   }
   if (a.res) {
-    float r[4];
-    load4_at<DT>(a.res, m * a.ldr + n, cnt, r);
+    float r[N];
+    load_at<DT>(a.res, m * a.ldr + n, cnt, r);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += r[j];
+    for (int j = 0; j < N; ++j) v[j] += r[j];
   }
-  store4_at<DT>(a.y, m * a.n + n, cnt, v);
+  store_at<DT>(a.y, m * a.n + n, cnt, v);
 }
-template <int DT>
-__device__ __forceinline__ void finish_glu(const DenseArgs& a, int64_t m, int64_t n, f32x4 g, f32x4 u, int cnt) {
+template <int DT, int N>
+__device__ __forceinline__ void finish_glu(const DenseArgs& a, int64_t m, int64_t n, const float (&g)[N], const float (&u)[N], int cnt) {
   if (a.z) {
-    const float gv[4] = {g[0], g[1], g[2], g[3]}, uv[4] = {u[0], u[1], u[2], u[3]};
-    store4_at<BCFFT_F32>(a.z, m * a.n + n, cnt, gv);
-    store4_at<BCFFT_F32>(a.z + a.m * a.n, m * a.n + n, cnt, uv);
+    store_at<BCFFT_F32>(a.z, m * a.n + n, cnt, g);
+    store_at<BCFFT_F32>(a.z + a.m * a.n, m * a.n + n, cnt, u);
   }
-  float h[4];
+  float h[N];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) h[j] = act_value(a.act, g[j]) * u[j];
-  store4_at<DT>(a.y, m * a.n + n, cnt, h);
+  for (int j = 0; j < N; ++j) h[j] = act_value(a.act, g[j]) * u[j];
+  store_at<DT>(a.y, m * a.n + n, cnt, h);
 }
 
 // partial sums of a slice of k: rows of 2 n for the gated form, whose `n` here counts both halves
 __device__ __forceinline__ int64_t partial_width(const DenseArgs& a) { return a.b[1] && a.segs == 1 ? 2 * a.n : a.n; }
-__device__ __forceinline__ void store_partial(const DenseArgs& a, int slice, int64_t m, int64_t n, f32x4 acc, int cnt) {
-  const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-  store4_at<BCFFT_F32>(a.ws, ((int64_t)slice * a.m + m) * partial_width(a) + n, cnt, v);
+template <int N>
+__device__ __forceinline__ void store_partial(const DenseArgs& a, int slice, int64_t m, int64_t n, const float (&v)[N], int cnt) {
+  store_at<BCFFT_F32>(a.ws, ((int64_t)slice * a.m + m) * partial_width(a) + n, cnt, v);
 }
-__device__ __forceinline__ f32x4 load_partials(const DenseArgs& a, int64_t m, int64_t n, int cnt) {
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < a.kz; ++k) {
-    float v[4];
-    load4_at<BCFFT_F32>(a.ws, ((int64_t)k * a.m + m) * partial_width(a) + n, cnt, v);
+template <int N>
+__device__ __forceinline__ void load_partials(const DenseArgs& a, int64_t m, int64_t n, int cnt, float (&s)[N]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] += v[j];
+  for (int j = 0; j < N; ++j) s[j] = 0.f;
+  for (int k = 0; k < a.kz; ++k) {
+    float v[N];
+    load_at<BCFFT_F32>(a.ws, ((int64_t)k * a.m + m) * partial_width(a) + n, cnt, v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[j] += v[j];
   }
-  return s;
 }
 
 }  // namespace bcfft

@@ -31,9 +31,9 @@ __global__ __launch_bounds__(256) void bc_dense_dz_kernel(DzArgs a) {
       const int64_t m = m0 + 4 * r + lane;
       if (m >= a.m) break;
       float d[4], z[4];
-      load4_at<DT>(a.dy, m * a.ldd + n, cnt, d);
+      load_at<DT>(a.dy, m * a.ldd + n, cnt, d);
       if (a.z) {
-        load4_at<BCFFT_F32>(a.z, m * a.n + n, cnt, z);
+        load_at<BCFFT_F32>(a.z, m * a.n + n, cnt, z);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float s, v;
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void bc_dense_dz_kernel(DzArgs a) {
           d[j] *= s;
         }
       }
-      if (a.dz) store4_at<DT>(a.dz, m * a.ldz + n, cnt, d);
+      if (a.dz) store_at<DT>(a.dz, m * a.ldz + n, cnt, d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[j] += d[j];
     }
@@ -73,8 +73,8 @@ __global__ __launch_bounds__(256) void bc_dense_db_kernel(const float* __restric
   if (lane == 0 && i < n) {
 #pragma unroll
     for (int k = 1; k < 8; ++k) s += sums[k][c];
-    const float v[4] = {(float)s, 0.f, 0.f, 0.f};
-    store4_at<DT>(db, i, 1, v);
+    const float v[1] = {(float)s};
+    store_at<DT>(db, i, 1, v);
   }
 }
 // dg = dh u act'(g) and du = dh act(g), side by side in a row
@@ -85,9 +85,9 @@ __global__ __launch_bounds__(256) void bc_dense_dgu_kernel(DzArgs a) {
     const int64_t m = q / quads, n = (q - m * quads) * 4;
     const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
     float d[4], g[4], u[4], dg[4], du[4];
-    load4_at<DT>(a.dy, m * a.ldd + n, cnt, d);
-    load4_at<BCFFT_F32>(a.z, m * a.n + n, cnt, g);
-    load4_at<BCFFT_F32>(a.z + a.m * a.n, m * a.n + n, cnt, u);
+    load_at<DT>(a.dy, m * a.ldd + n, cnt, d);
+    load_at<BCFFT_F32>(a.z, m * a.n + n, cnt, g);
+    load_at<BCFFT_F32>(a.z + a.m * a.n, m * a.n + n, cnt, u);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float s, v;
@@ -95,8 +95,8 @@ __global__ __launch_bounds__(256) void bc_dense_dgu_kernel(DzArgs a) {
       dg[j] = d[j] * u[j] * s;
       du[j] = d[j] * v;
     }
-    store4_at<DT>(a.dz, m * a.ldz + n, cnt, dg);
-    store4_at<DT>(a.dz, m * a.ldz + a.ldz / 2 + n, cnt, du);
+    store_at<DT>(a.dz, m * a.ldz + n, cnt, dg);
+    store_at<DT>(a.dz, m * a.ldz + a.ldz / 2 + n, cnt, du);
   }
 }
 
@@ -116,14 +116,15 @@ __global__ __launch_bounds__(256) void bc_dense_pack_kernel(const char* __restri
 
 // ------------------------------------------------------------------ launches
 // Tile and slices for an m x n product over ksteps tiles of k, with `parts` products per output (2: gated):
-// the least estimated time in microseconds. step: one tile of k of one workgroup with its CU's share (16-bit:
-// measured at 8192 x 4096 x 4096; fp32: the fp32 matrix rate). Slices pay their partial sums' way through
-// memory and the finishing launch.
-static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, bool forward) {
-  if (forward && m <= 32) return {0, 1};
+// the least estimated time in microseconds. step: one tile of k of one workgroup with its CU's share, fixed: its
+// start and its outputs (16-bit: measured at 8192 x 4096 x 4096, 2048 x 4096 x 64 to 4096 and, by columns,
+// 22016 x 4096 x 1700; fp32: the fp32 matrix rate). cols: operands that lie by columns (256 x 128 tiles read
+// theirs in rows of 256 bytes). Slices pay their partial sums' way through memory and the finishing launch.
+static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int cols) {
+  if (cols == 0 && m <= 32) return {0, 1};
   const int64_t cus = device_cu_count();
   struct Kind { int kind, bm, bn, slots; double step, step32, fixed; };
-  const Kind kinds[3] = {{1, 128, 128, 2, 0.48, 1.9, 3.0}, {2, 256, 128, 1, 0.80, 3.8, 5.0}, {3, 256, 256, 1, 1.55, 7.6, 8.0}};
+  const Kind kinds[3] = {{1, 128, 128, 2, 0.48, 1.9, 2.5}, {2, 256, 128, 1, 0.82 + 0.06 * cols, 3.7, 3.0}, {3, 256, 256, 1, 1.55, 7.3, 6.0}};
   Shape best{1, 1};
   double least = 1e300;
   for (const Kind& q : kinds) {
@@ -185,7 +186,7 @@ struct ForwardPlan {
 };
 static ForwardPlan forward_plan(int64_t n, int64_t k, int64_t m, int dt, int parts) {
   ForwardPlan p;
-  p.shape = choose(n, m, ksteps(k, dt), parts, dt, true);
+  p.shape = choose(n, m, ksteps(k, dt), parts, dt, 0);
   p.packed = p.shape.kind != 0 && !whole(k, dt);       // the few-rows kernel reads any address
   p.pack_bytes = p.packed ? packed_bytes(n + parts * m, k, dt) : 0;
   p.total = p.pack_bytes + partial_bytes(n, parts * m, p.shape);
@@ -199,8 +200,8 @@ struct BackwardPlan {                                  // workspace of a backwar
 static BackwardPlan backward_plan(int64_t n, int64_t k, int64_t m, int dt, int parts, int act) {
   BackwardPlan p;
   const bool split = parts == 2 && !whole(m, dt);      // dg and du are not adjacent columns
-  p.dx = choose(n, k, parts * ksteps(m, dt), 1, dt, false);
-  p.dw = choose(split ? m : parts * m, k, ksteps(n, dt), 1, dt, false);
+  p.dx = choose(n, k, parts * ksteps(m, dt), 1, dt, 1);
+  p.dw = choose(split ? m : parts * m, k, ksteps(n, dt), 1, dt, 2);
   p.dz_bytes = parts == 2 || act != BCFFT_ACT_NONE || !whole(m, dt) ? parts * packed_bytes(n, m, dt) : 0;
   // 64 rows per workgroup of dz where that makes four workgroups per CU, else 16 (2048 x 4096: 25 -> 18 us, 1362 x 448: 18 -> 6 us)
   p.rows = (n + 63) / 64 * ((m + 255) / 256) >= 4 * device_cu_count() ? 64 : 16;

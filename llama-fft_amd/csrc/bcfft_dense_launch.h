@@ -14,9 +14,14 @@ __global__ __launch_bounds__(256) void bc_dense_finish_kernel(DenseArgs a) {
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
     const int64_t m = q / quads, n = (q - m * quads) * 4;
     const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
-    f32x4 g = load_partials(a, m, n, cnt);
-    if constexpr (GLU) finish_glu<DT>(a, m, n, g, load_partials(a, m, a.n + n, cnt), cnt);
-    else finish_linear<DT>(a, m, n, g, cnt);
+    float g[4], u[4];
+    load_partials(a, m, n, cnt, g);
+    if constexpr (GLU) {
+      load_partials(a, m, a.n + n, cnt, u);
+      finish_glu<DT>(a, m, n, g, u, cnt);
+    } else {
+      finish_linear<DT>(a, m, n, g, cnt);
+    }
   }
 }
 
@@ -94,12 +99,14 @@ __global__ __launch_bounds__(64 * KW) void bc_dense_rows_kernel(DenseArgs a) {
   for (int i = wave; i < MT; i += KW) {
     const int64_t m = 16 * i + l, n = n0 + 4 * g;
     if (m >= a.m || n >= a.n) continue;
-    f32x4 v[NB];
+    float v[NB][4];
 #pragma unroll
     for (int s = 0; s < NB; ++s) {
-      v[s] = part[0][s * MT + i][lane];
+      f32x4 sum = part[0][s * MT + i][lane];
 #pragma unroll
-      for (int w = 1; w < KW; ++w) v[s] += part[w][s * MT + i][lane];
+      for (int w = 1; w < KW; ++w) sum += part[w][s * MT + i][lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[s][j] = sum[j];
     }
     const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
     if constexpr (GLU) finish_glu<DT>(a, m, n, v[0], v[NB - 1], cnt);

@@ -347,28 +347,45 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void bc_dense_tile_kernel(DenseArg
     }
   }
 
-  // lane: row m0 + .. + (lane & 15), four consecutive columns from 4 (lane >> 4)
+  // The accumulators of 16 rows at a time through the wave's own piece of LDS (its buffers are free, and a
+  // wave's LDS accesses are in order), so that a lane finishes eight consecutive columns and a row's columns of
+  // this wave are stored as whole lines (16 rows x 64 columns: 8 rows of 128 bytes per store; as they lie in
+  // the accumulators 16 rows of 32 bytes: 256 x 256 tiles of k = 64 took 19.1 us, 12.7 so)
+  constexpr int OC = TN / NB, PITCH = TN + 4, LPR = OC / 8, RPP = 64 / LPR;
+  static_assert(WM * WN * 16 * PITCH * 4 <= RA * ABYTES + RB * BBYTES && 16 % RPP == 0, "the waves' pieces of LDS");
+  float* const st = (float*)lds + wave * 16 * PITCH;
+  const int r0 = lane / LPR, c0 = lane % LPR * 8;
+  const int64_t n = n0 + wn * OC + c0;
+  const int cnt = n < a.n ? (a.n - n < 8 ? (int)(a.n - n) : 8) : 0;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int64_t m = m0 + wm * TM + i * 16 + (lane & 15);
-    if (m >= a.m) continue;
 #pragma unroll
-    for (int j = 0; j < FN / NB; ++j) {
-      const int64_t n = n0 + wn * (TN / NB) + j * 16 + 4 * (lane >> 4);
-      if (n >= a.n) continue;
-      const int cnt = a.n - n < 4 ? (int)(a.n - n) : 4;
-      if constexpr (GLU) {
+    for (int j = 0; j < FN; ++j) *reinterpret_cast<f32x4*>(st + (lane & 15) * PITCH + j * 16 + 4 * (lane >> 4)) = acc[i][j];
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int p = 0; p < 16 / RPP; ++p) {
+      const int r = p * RPP + r0;
+      const int64_t m = m0 + wm * TM + i * 16 + r;
+      float v[8], u[8];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(st + r * PITCH + c0 + 4 * q);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(st + r * PITCH + (GLU ? OC : 0) + c0 + 4 * q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * q + j] = x[j], u[4 * q + j] = y[j];
+      }
+      if (m < a.m && cnt > 0) {
         if (a.kz > 1) {
-          store_partial(a, blockIdx.y, m, n, acc[i][j], cnt);
-          store_partial(a, blockIdx.y, m, a.n + n, acc[i][j + FN / 2], cnt);
+          store_partial(a, blockIdx.y, m, n, v, cnt);
+          if constexpr (GLU) store_partial(a, blockIdx.y, m, a.n + n, u, cnt);
+        } else if constexpr (GLU) {
+          finish_glu<DT>(a, m, n, v, u, cnt);
         } else {
-          finish_glu<DT>(a, m, n, acc[i][j], acc[i][j + FN / 2], cnt);
+          finish_linear<DT>(a, m, n, v, cnt);
         }
-      } else {
-        if (a.kz > 1) store_partial(a, blockIdx.y, m, n, acc[i][j], cnt);
-        else finish_linear<DT>(a, m, n, acc[i][j], cnt);
       }
     }
+    asm volatile("" ::: "memory");
   }
 }
 
