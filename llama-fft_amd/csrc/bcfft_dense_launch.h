@@ -29,7 +29,10 @@ __global__ __launch_bounds__(256) void bc_dense_finish_kernel(DenseArgs a) {
 // Up to 16 MT rows of x (decode): bound by the weights' single read. A workgroup takes 16 rows of W (and 16
 // of the other weight, GLU), its KW waves a part of k each, straight from memory into the fragments; x comes
 // out of L2. The waves' sums meet in LDS.
-template <int DT, int MT, int KW, bool GLU>
+// A wave with few 128-byte tiles of k (8 for 4096 16-bit values) loads four at a time; with more (STREAM) it
+// loads one while it multiplies the last: 1 x 4096 -> 2 x 11008 36.9 us against 34.1 from HBM (5.3 TB/s), 1 x
+// 11008 -> 4096 22.7 against 20.3, but 1 x 4096 -> 4096 6.6 against 7.0 and every two-row-tile form.
+template <int DT, int MT, int KW, bool STREAM, bool GLU>
 __global__ __launch_bounds__(64 * KW) void bc_dense_rows_kernel(DenseArgs a) {
   constexpr int E = DT == BCFFT_F32 ? 4 : 2, EPC = 16 / E, BK = 128 / E, NB = GLU ? 2 : 1;
   constexpr int UNROLL = 4;
@@ -62,22 +65,56 @@ __global__ __launch_bounds__(64 * KW) void bc_dense_rows_kernel(DenseArgs a) {
       for (int i = 0; i < MT; ++i) acc[s][i] = mma<DT>(w[s], x[i], acc[s][i]);
   };
   int64_t t = t0;
-  for (; t + UNROLL <= t1 && (t + UNROLL) * BK <= a.k; t += UNROLL) {
-    uint4 w[UNROLL][2][NB], x[UNROLL][2][MT];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
+  if constexpr (STREAM) {
+    const int64_t whole = a.k / BK < t1 ? a.k / BK : t1;
+    uint4 w[2][2][NB], x[2][2][MT];
+    auto fill = [&](int buf, int64_t tile) {
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        const int64_t k = (t + u) * BK + (g + 4 * kk) * EPC;
+        const int64_t k = tile * BK + (g + 4 * kk) * EPC;
 #pragma unroll
-        for (int s = 0; s < NB; ++s) w[u][kk][s] = load(pw[s], k);
+        for (int s = 0; s < NB; ++s) w[buf][kk][s] = load(pw[s], k);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) x[u][kk][i] = load(px[i], k);
+        for (int i = 0; i < MT; ++i) x[buf][kk][i] = load(px[i], k);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto use = [&](int buf) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
+      for (int kk = 0; kk < 2; ++kk) step(w[buf][kk], x[buf][kk]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (t < whole) {
+      fill(0, t);
+      for (; t + 2 <= whole; t += 2) {
+        fill(1, t + 1);
+        use(0);
+        fill(0, t + 2 < whole ? t + 2 : whole - 1);    // past the end the last one again, unused
+        use(1);
+      }
+      if (t < whole) {
+        use(0);
+        ++t;
+      }
+    }
+  } else {
+    for (; t + UNROLL <= t1 && (t + UNROLL) * BK <= a.k; t += UNROLL) {
+      uint4 w[UNROLL][2][NB], x[UNROLL][2][MT];
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) step(w[u][kk], x[u][kk]);
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const int64_t k = (t + u) * BK + (g + 4 * kk) * EPC;
+#pragma unroll
+          for (int s = 0; s < NB; ++s) w[u][kk][s] = load(pw[s], k);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) x[u][kk][i] = load(px[i], k);
+        }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) step(w[u][kk], x[u][kk]);
+    }
   }
   for (; t < t1; ++t) {
 #pragma unroll
@@ -146,14 +183,26 @@ static void launch_tiles(const DenseArgs& a, int kind, hipStream_t s) {
 template <int DT, bool GLU>
 static void launch_rows(const DenseArgs& a, hipStream_t s) {
   const unsigned groups = (unsigned)((a.n + 15) / 16);
-  auto go = [&](auto mt, auto kw) {
-    hipLaunchKernelGGL((bc_dense_rows_kernel<DT, mt.value, kw.value, GLU>), dim3(groups), dim3(64 * kw.value), 0, s, a);
+  const int64_t tiles = (a.k * (DT == BCFFT_F32 ? 4 : 2) + 127) / 128;
+  auto go = [&](auto mt, auto kw, auto stream) {
+    hipLaunchKernelGGL((bc_dense_rows_kernel<DT, mt.value, kw.value, stream.value, GLU>), dim3(groups), dim3(64 * kw.value), 0, s, a);
   };
   using std::integral_constant;
-  if (a.m <= 16 && groups <= 512) go(integral_constant<int, 1>(), integral_constant<int, 8>());
-  else if (a.m <= 16) go(integral_constant<int, 1>(), integral_constant<int, 4>());
-  else if (groups <= 512) go(integral_constant<int, 2>(), integral_constant<int, 8>());
-  else go(integral_constant<int, 2>(), integral_constant<int, 4>());
+  using std::bool_constant;
+  const integral_constant<int, 1> one;
+  const integral_constant<int, 2> two;
+  const integral_constant<int, 4> kw4;
+  const integral_constant<int, 8> kw8;
+  // 8 waves per 16 rows of W while that leaves no more than two workgroups per CU, 4 beyond
+  if (groups <= 512) {
+    if (a.m > 16) go(two, kw8, bool_constant<false>());
+    else if (tiles >= 12 * 8) go(one, kw8, bool_constant<true>());
+    else go(one, kw8, bool_constant<false>());
+  } else {
+    if (a.m > 16) go(two, kw4, bool_constant<false>());
+    else if (tiles >= 12 * 4) go(one, kw4, bool_constant<true>());
+    else go(one, kw4, bool_constant<false>());
+  }
 }
 
 template <int DT>
