@@ -27,25 +27,20 @@ namespace bcfft {
 constexpr int TOPK_MAX = 1024;          // entries per row
 constexpr int DISTILL_VOCAB_MAX = 1 << 18;   // the entries' bitmap: 32 KB of LDS
 
-// exp((v - ref) / T) as exp2(v c + v lo + b), b = -ref c rounded: c + lo = log2(e) / T to 48 bits, so the
-// constant's own rounding (up to 3e-8 relative, times v: the same sign in every term) does not shift the
-// sum; b's rounding multiplies every term alike and is taken out of the sums in fp64 (drift).
-// c is rounded down and lo > 0: for v = -inf both products are -inf, never inf - inf.
+// exp((v - ref) / T) as exp2(x c + x lo), x = v - ref: c + lo = log2(e) / T to 48 bits, so the constant's own
+// rounding (up to 3e-8 relative, times x: the same sign in every term) does not shift the sum. c is rounded
+// down and lo > 0: for x = -inf both products are -inf, never inf - inf. The difference is taken first: with
+// ref = the type's lowest value (a row masked by it alone) ref c would overflow.
 struct ExpScale {
   float c, lo;
 };
-__device__ __forceinline__ float exp_at(float v, ExpScale e, float b) {
-  return __builtin_amdgcn_exp2f(fmaf(v, e.lo, fmaf(v, e.c, b)));
+__device__ __forceinline__ float exp_at(float v, ExpScale e, float ref) {
+  const float x = v - ref;
+  return __builtin_amdgcn_exp2f(fmaf(x, e.c, x * e.lo));
 }
-// the same without lo: the constant's rounding is taken out at ref alone, which leaves it times the distance
-// from ref (at most as much as the argument's own rounding)
-__device__ __forceinline__ float exp_near(float v, ExpScale e, float b) { return __builtin_amdgcn_exp2f(fmaf(v, e.c, b)); }
-__device__ __forceinline__ float exp_base(float ref, ExpScale e) { return -ref * e.c; }
-// log2 of what exp_at's (drift_near: at v = ref, exp_near's) values are too large by
-__device__ __forceinline__ double drift(float ref, ExpScale e, float b) {
-  return (double)b + (double)ref * ((double)e.c + (double)e.lo);
-}
-__device__ __forceinline__ double drift_near(float ref, ExpScale e, float b) { return (double)b + (double)ref * (double)e.c; }
+// the same without lo, for sums whose terms lie near ref: what is left of the constant's rounding is at most
+// as much as the argument's own
+__device__ __forceinline__ float exp_near(float v, ExpScale e, float ref) { return __builtin_amdgcn_exp2f((v - ref) * e.c); }
 
 template <int DT> struct RowType {
   static constexpr int VEC = 8;        // elements per 16 bytes
@@ -245,7 +240,6 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
   // an element reaches the bound unless it is less: NaN does, and without a bound all do
   const uint32_t bound_key = (uint32_t)bound_s << 16;
   const float bound = bound_key ? key_value(bound_key) : -INFINITY;
-  const float base = exp_base(bound, es);
   float s = 0.f;
   // one bit per logit of a thread that reaches the bound, listed after the pass: no branch in it
   uint64_t reach = 0;
@@ -266,7 +260,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
 #pragma unroll
       for (int j = N - 1; j >= 0; --j) {
         const bool under = v[j] < bound;
-        s += under ? exp_near(v[j], es, base) : 0.f;
+        s += under ? exp_near(v[j], es, bound) : 0.f;
         m = m << 1 | (under ? 0 : 1);
       }
       if (bit == 0) first = at / VEC;
@@ -281,7 +275,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
       list();                            // what the pieces left, then the element behind them
       reach = 0;
       if (v[0] < bound) {
-        s += exp_near(v[0], es, base);
+        s += exp_near(v[0], es, bound);
       } else {
         const int p = atomicAdd(&count, 1);
         if (p < TOPK_CAND) at_s[p] = at;
@@ -293,7 +287,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
   const double sum = block_reduce<NT>((double)s, redd, SumOp());
   int m = count;
   const bool flood = m > TOPK_CAND;      // uniform over the workgroup, as all that follows from it
-  double log_under = sum > 0.0 ? (log2(sum) - drift_near(bound, es, base)) * 0.6931471805599453 + (double)bound * inv_t : -INFINITY;
+  double log_under = sum > 0.0 ? log(sum) + (double)bound * inv_t : -INFINITY;
   if (flood || !(sum > 1e-20 && sum < 1e30)) {
     // the exact cut: an element is taken up if key > cut_key, or key == cut_key at an index up to cut_index
     uint32_t cut_key = bound_key;
@@ -335,18 +329,18 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
       }
     });
     below = block_reduce<NT>(below, redf, MaxOp());
-    const float ref = below == -INFINITY ? 0.f : below, b2 = exp_base(ref, es);
+    const float ref = below == -INFINITY ? 0.f : below;
     float s2 = 0.f;
     r.each([&](int at, auto& v) {
 #pragma unroll
       for (int j = 0; j < count_of<decltype(v)>; ++j) {
         const uint32_t key = order_key(v[j]);
         const bool taken = key > cut_key || (key == cut_key && at <= cut_index - j);
-        s2 += taken ? 0.f : exp_at(v[j], es, b2);
+        s2 += taken ? 0.f : exp_at(v[j], es, ref);
       }
     });
     const double sum2 = block_reduce<NT>((double)s2, redd, SumOp());
-    log_under = (log2(sum2) - drift(ref, es, b2)) * 0.6931471805599453 + (double)ref * inv_t;   // log 0 = -inf
+    log_under = log(sum2) + (double)ref * inv_t;       // log 0 = -inf: nothing left
     if (flood) m = k;
   }
 
@@ -510,7 +504,7 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, int64_t n, E
 }
 // The other elements': exp((v - ref) / T) times coef
 template <int DT, class ROW>
-__device__ __forceinline__ void write_others(const DistillArgs& a, int64_t n, ROW& r, const uint32_t* bits, float base,
+__device__ __forceinline__ void write_others(const DistillArgs& a, int64_t n, ROW& r, const uint32_t* bits, float ref,
                                              float coef) {
   char* out = (char*)a.grad + n * a.vocab * (DT == BCFFT_F32 ? 4 : 2);
   r.each([&](int at, auto& v) {
@@ -518,7 +512,7 @@ __device__ __forceinline__ void write_others(const DistillArgs& a, int64_t n, RO
     const uint32_t keep = ~piece_bits<N>(bits, at);
     float g[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) g[j] = unless(keep, j, exp_at(v[j], a.es, base) * coef);
+    for (int j = 0; j < N; ++j) g[j] = unless(keep, j, exp_at(v[j], a.es, ref) * coef);
     store_piece<DT>(out, at, g);
   });
 }
@@ -580,7 +574,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
     if constexpr (GRAD) write_zero<DT, NT>(a, n);
     return;
   }
-  const float m_all = mx == -INFINITY ? 0.f : mx, base = exp_base(m_all, a.es);
+  const float m_all = mx == -INFINITY ? 0.f : mx;
 
   // sums over the entries: the teacher's total, the student's, the loss's part linear in the logits. Before
   // the pass over the row: fp64 functions take 40 registers
@@ -614,14 +608,14 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
         const uint32_t keep = ~piece_bits<VEC>(bits, p * VEC);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          kept[i][j] = unless(keep, j, exp_at(v[j], a.es, base));
+          kept[i][j] = unless(keep, j, exp_at(v[j], a.es, m_all));
           so += kept[i][j];
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (tid < r.tail) {
-      kept_tail = unless(~piece_bits<1>(bits, (int)(r.pieces * VEC) + tid), 0, exp_at(r.last, a.es, base));
+      kept_tail = unless(~piece_bits<1>(bits, (int)(r.pieces * VEC) + tid), 0, exp_at(r.last, a.es, m_all));
       so += kept_tail;
     }
   } else {
@@ -629,7 +623,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
       constexpr int N = count_of<decltype(v)>;
       const uint32_t keep = ~piece_bits<N>(bits, at);
 #pragma unroll
-      for (int j = 0; j < N; ++j) so += unless(keep, j, exp_at(v[j], a.es, base));
+      for (int j = 0; j < N; ++j) so += unless(keep, j, exp_at(v[j], a.es, m_all));
     });
   }
   double sums[4] = {(double)so, total, se, lin};
@@ -644,7 +638,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
   for (int q = 0; q < 4; ++q) sums[q] = across_waves<NT>(en.redd[q], SumOp());
   const double rest_a = a.rest ? (double)a.rest[n] - am : -INFINITY, rest_e = exp(rest_a);
   const double inv_total = 1.0 / (sums[1] + rest_e), rest_p = rest_e * inv_total;
-  double sum_o = sums[0] * exp2(-drift(m_all, a.es, base));      // relative to m_all
+  double sum_o = sums[0];                // relative to m_all
   const double sum_e = sums[2];
   float ref = m_all;
   double sum_ref = sum_o;                // the others' sum relative to ref
@@ -661,15 +655,14 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
     });
     mo = block_reduce<NT>(mo, en.redf, MaxOp());
     ref = mo == -INFINITY ? 0.f : mo;
-    const float b2 = exp_base(ref, a.es);
     float s2 = 0.f;
     r2.each([&](int at, auto& v) {
       constexpr int N = count_of<decltype(v)>;
       const uint32_t keep = ~piece_bits<N>(bits, at);
 #pragma unroll
-      for (int j = 0; j < N; ++j) s2 += unless(keep, j, exp_at(v[j], a.es, b2));
+      for (int j = 0; j < N; ++j) s2 += unless(keep, j, exp_at(v[j], a.es, ref));
     });
-    sum_ref = block_reduce<NT>((double)s2, en.topd, SumOp()) * exp2(-drift(ref, a.es, b2));
+    sum_ref = block_reduce<NT>((double)s2, en.topd, SumOp());
     sum_o = mo == -INFINITY ? 0.0 : sum_ref * exp(((double)ref - (double)m_all) * a.inv_t);
   }
   const double sum = sum_o + sum_e, inv_s = 1.0 / sum;
@@ -687,7 +680,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
     const float scale = (float)(w * a.inv_t);
     if (KEEP && !again) {
       char* out = (char*)a.grad + n * a.vocab * E;
-      const float c = (float)(coef * exp2(-drift(m_all, a.es, base))) * scale;
+      const float c = (float)coef * scale;
 #pragma unroll
       for (int i = 0; i < (KEEP ? HOLD : 0); ++i) {
         const int p = i * NT + tid;
@@ -700,13 +693,13 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
       }
       if (tid < r.tail) store_one<DT>(out, r.pieces * VEC + tid, kept_tail * c);
     } else {
-      const float b = exp_base(ref, a.es), c = (float)(coef * exp2(-drift(ref, a.es, b))) * scale;
+      const float c = (float)coef * scale;
       if (HOLD > 0 && !KEEP) {
-        write_others<DT>(a, n, r, bits, b, c);
+        write_others<DT>(a, n, r, bits, ref, c);
       } else {
         Row<DT, NT, 0> r2;
         r2.open(row, a.vocab);
-        write_others<DT>(a, n, r2, bits, b, c);
+        write_others<DT>(a, n, r2, bits, ref, c);
       }
     }
     write_entries<DT, NT>(a, n, en, m_all, inv_s, inv_total, scale);
@@ -736,10 +729,10 @@ __global__ __launch_bounds__(NT) void bc_distill_backward_kernel(DistillArgs a) 
   }
   total = block_reduce<NT>(total, en.topd, SumOp()) + (a.rest ? exp((double)a.rest[n] - am) : 0.0);
   const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * n);
-  const float scale = (float)(w * a.inv_t) * a.upstream[n], base = exp_base(st.x, a.es);
+  const float scale = (float)(w * a.inv_t) * a.upstream[n];
   Row<DT, NT, 0> r;
   r.open(row, a.vocab);
-  write_others<DT>(a, n, r, bits, base, st.y * (float)exp2(-drift(st.x, a.es, base)) * scale);
+  write_others<DT>(a, n, r, bits, st.x, st.y * scale);
   write_entries<DT, NT>(a, n, en, st.z, st.w, 1.0 / total, scale);
 }
 

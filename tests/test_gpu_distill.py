@@ -74,7 +74,8 @@ def kl_oracle(s, values, indices, rest, weight, t):
         if p[-1] > 0:
             total += float(p[-1] * (logp[-1] - log_rest))
             if log_rest > NEG:
-                share = p[-1] * torch.exp(logq[others] - log_rest)
+                # exp(logq - log_rest); both may be near -3e38, where a double no longer holds log(count)
+                share = p[-1] * torch.softmax(s[i][others] / t, 0)
                 g[others] -= share
                 m[others] += share
         loss[i], grad[i], size[i] = total * w, g * (w / t), m * abs(w / t)
@@ -401,3 +402,53 @@ def test_ctypes_path_is_identical(dev, monkeypatch):
             mp.setattr(_lib, "_native", False)
             other = all_of()
         assert all(p.shape == q.shape and p.dtype == q.dtype and torch.equal(p, q) for p, q in zip(native, other))
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_rows_masked_by_the_lowest_value(dev, dt):
+    """Masks of the type's lowest value instead of -inf: alone, beside real logits, and with -inf under them."""
+    from bcfft import distill
+    low = torch.finfo(DT[dt]).min
+    v = 3000
+    z = torch.full((5, v), low)
+    z[1, :10] = torch.arange(10.0)
+    z[2, 5] = 3.0
+    z[2, 100:] = NEG
+    z[3, 7:] = NEG
+    z[4] = -z[4]                                      # and the largest value
+    z[4, 9:] = 0.0
+    z = z.to(DT[dt])
+    for k in (1, 4, 12, 200):
+        values, indices, rest = distill.topk_logits(z.to(dev), k)
+        top, want = teacher_oracle(z, k, 1.0)
+        assert torch.equal(indices.cpu().long(), top) and torch.equal(values.cpu(), z.gather(-1, top))
+        rest = rest.double().cpu()
+        fine = want.abs() < 3e38                      # (lowest + log(v) itself may not be a finite fp32)
+        assert bool(((rest - want).abs() <= LOG_TOL + 2.0 ** -23 * want.abs())[fine & torch.isfinite(want)].all())
+        assert torch.equal(rest == NEG, want < -3.4028235e38)
+    top = torch.tensor([[0, 1, 5], [0, 1, 50], [5, 6, 7], [0, 1, 2], [20, 21, 2]])
+    vals = torch.tensor([[1.0, 0.5, 0.25]]).expand(5, 3).contiguous()
+    for rest in (None, torch.zeros(5)):
+        want, dwant, size = kl_oracle(z, vals, top, rest, None, 1.0)
+        loss, grad = distill.topk_kl_grad(z.to(dev), vals.to(dev), top.to(dev), rest=None if rest is None else rest.to(dev))
+        fine = want < 1e37
+        assert torch.equal(torch.isfinite(loss.cpu()) & (loss.cpu() < 1e37), fine)
+        check_loss(loss[fine.to(dev)], want[fine])
+        check_grad(grad, dwant, size)
+
+
+def test_extreme_temperatures(dev):
+    from bcfft import distill
+    s = logits_of(4, 700, torch.float32, seed=41, scale=5.0)
+    _, top, values = entries_of(s, 9, torch.float32, 42)
+    for t in (1e-6, 1e-3, 30.0, 1e6):
+        want, dwant, size = kl_oracle(s, values, top, None, None, t)
+        loss, grad = distill.topk_kl_grad(s.to(dev), values.to(dev), top.to(dev), temperature=t)
+        # a logit over T is rounded to fp32 before the exponential: 2^-24 of |s| / T where it counts
+        extra = 4 * 2.0 ** -24 * want.abs()
+        assert bool(((loss.double().cpu() - want).abs() <= 2 * LOG_TOL + 2.0 ** -23 * want.abs() + extra).all())
+        check_grad(grad, dwant, size)
+        v2, i2, rest = distill.topk_logits(s.to(dev), 9, t)
+        at, r = teacher_oracle(s, 9, t)
+        assert torch.equal(i2.cpu().long(), at)
+        assert bool(((rest.double().cpu() - r).abs() <= LOG_TOL + 2.0 ** -22 * r.abs()).all())
