@@ -179,9 +179,11 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 1. Each thread's largest logit; the k-th largest of these NT bounds the k-th largest element from below (k
-//    threads hold at least one that large each), and hardly more than k elements reach it (74 for k = 64
-//    of 256 threads, evenly spread). Its upper 16 bits are enough.                   1.5 operations a logit
+// 1. The largest logit of each thread or, for k <= 128, of each of 256 groups of threads; the k-th largest of
+//    these bounds the k-th largest element from below (k groups hold at least one that large each), and
+//    hardly more than k elements reach it (74 for k = 64 of 256, evenly spread). Its upper 16 bits are enough:
+//    one wave finds it bit by bit, by ballots over G / 64 maxima per lane (16 of them: 8000 of the kernel's
+//    29000 clocks at 20 x 32000, which is why there are no more than 4 where k allows it). 1.5 operations a logit
 // 2. The elements at or above the bound go to LDS, the others' exponentials relative to it are summed.    9
 // 3. Each candidate counts the candidates above it: its rank is its place in the output. Ranks depend on
 //    keys alone, so the order of arrival does not matter.
@@ -200,12 +202,13 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
   __shared__ uint64_t cand[TOPK_CAND];   // their keys
   __shared__ uint32_t raw[TOPK_CAND];    // their logits as they stand in the row
   __shared__ float left[TOPK_CAND];
-  __shared__ uint32_t tmax[NT];
+  __shared__ uint32_t gmax[NT];
   __shared__ uint32_t redu[NT / 64];
   __shared__ float redf[NT / 64];
   __shared__ double redd[NT / 64];
   __shared__ int count, bound_s;
   const int tid = threadIdx.x;
+  if (tid == 0) count = 0;
   const int64_t n = blockIdx.x;
   const char* row = (const char*)logits + n * row_stride * E;
   Row<DT, NT, HOLD> r;
@@ -219,22 +222,35 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
     for (int j = 0; j + 1 < count_of<decltype(v)>; j += 2) best = fmaxf(fmaxf(best, v[j]), v[j + 1]);
     if constexpr (count_of<decltype(v)> == 1) best = fmaxf(best, v[0]);
   });
-  tmax[tid] = any ? order_key(best) : 0;   // 0 is below every key of a number
-  if (tid == 0) count = 0;
+  // 0 is below every key of a number
+  uint32_t key = any ? order_key(best) : 0;
+  const bool grouped = NT > 256 && k <= 128;
+  if (grouped) {
+#pragma unroll
+    for (int d = 1; d < NT / 256; d *= 2) key = max(key, (uint32_t)__shfl_xor((int)key, d, 64));
+    if (tid % (NT / 256) == 0) gmax[tid / (NT / 256)] = key;
+  } else {
+    gmax[tid] = key;
+  }
   __syncthreads();
-  if (tid < 64) {                        // largest b with k thread maxima whose upper halves reach it
-    uint32_t mine[NT / 64];
+  if (tid < 64) {                        // largest b with k maxima whose upper halves reach it
+    auto search = [&](auto per_lane) {
+      uint32_t mine[per_lane.value];
 #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) mine[i] = tmax[i * 64 + tid] >> 16;
-    uint32_t b = 0;
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t trial = b | 1u << bit;
-      int c = 0;
+      for (int i = 0; i < per_lane.value; ++i) mine[i] = gmax[i * 64 + tid] >> 16;
+      uint32_t b = 0;
+      for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t trial = b | 1u << bit;
+        int c = 0;
 #pragma unroll
-      for (int i = 0; i < NT / 64; ++i) c += __popcll(__ballot(mine[i] >= trial));
-      if (c >= k) b = trial;
-    }
-    if (tid == 0) bound_s = (int)b;
+        for (int i = 0; i < per_lane.value; ++i) c += __popcll(__ballot(mine[i] >= trial));
+        if (c >= k) b = trial;
+        if (c == k) break;               // exactly k: lower bits only raise the bound between two maxima
+      }
+      if (tid == 0) bound_s = (int)b;
+    };
+    if (grouped) search(std::integral_constant<int, 4>());
+    else search(std::integral_constant<int, NT / 64>());
   }
   __syncthreads();
   // an element reaches the bound unless it is less: NaN does, and without a bound all do
@@ -287,7 +303,9 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
   const double sum = block_reduce<NT>((double)s, redd, SumOp());
   int m = count;
   const bool flood = m > TOPK_CAND;      // uniform over the workgroup, as all that follows from it
-  double log_under = sum > 0.0 ? log(sum) + (double)bound * inv_t : -INFINITY;
+  // the mass that is left, as log(under) + ref / T
+  double under = sum;
+  float ref = bound;
   if (flood || !(sum > 1e-20 && sum < 1e30)) {
     // the exact cut: an element is taken up if key > cut_key, or key == cut_key at an index up to cut_index
     uint32_t cut_key = bound_key;
@@ -329,7 +347,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
       }
     });
     below = block_reduce<NT>(below, redf, MaxOp());
-    const float ref = below == -INFINITY ? 0.f : below;
+    ref = below == -INFINITY ? 0.f : below;
     float s2 = 0.f;
     r.each([&](int at, auto& v) {
 #pragma unroll
@@ -339,8 +357,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
         s2 += taken ? 0.f : exp_at(v[j], es, ref);
       }
     });
-    const double sum2 = block_reduce<NT>((double)s2, redd, SumOp());
-    log_under = log(sum2) + (double)ref * inv_t;       // log 0 = -inf: nothing left
+    under = block_reduce<NT>((double)s2, redd, SumOp());
     if (flood) m = k;
   }
 
@@ -353,38 +370,42 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
     cand[i] = full_key(order_key(DT == BCFFT_F32 ? __uint_as_float(u) : unpack16<DT == BCFFT_F32 ? BCFFT_BF16 : DT>(u).x), at);
   }
   __syncthreads();
-  for (int i = tid; i < m; i += NT) {
-    const uint64_t key = cand[i];
+  // 16 lanes per candidate: each compares it with every 16th
+  for (int i = tid / 16; i < (m + 3) / 4 * 4; i += NT / 16) {      // whole waves: they shuffle
+    const uint64_t key = cand[i < m ? i : 0];
     int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < m; ++j) rank += cand[j] > key;
-    if (rank < k) {
-      if constexpr (DT == BCFFT_F32) ((uint32_t*)values)[n * k + rank] = raw[i];
-      else ((uint16_t*)values)[n * k + rank] = (uint16_t)raw[i];
-      indices[n * k + rank] = (int32_t)~(uint32_t)key;
-    } else {
-      left[rank] = key_value((uint32_t)(key >> 32));
+#pragma unroll 4
+    for (int j = tid % 16; j < m; j += 16) rank += cand[j] > key;
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) rank += __shfl_xor(rank, d, 64);
+    if (i < m && tid % 16 == 0) {
+      if (rank < k) {
+        if constexpr (DT == BCFFT_F32) ((uint32_t*)values)[n * k + rank] = raw[i];
+        else ((uint16_t*)values)[n * k + rank] = (uint16_t)raw[i];
+        indices[n * k + rank] = (int32_t)~(uint32_t)key;
+      } else {
+        left[rank] = key_value((uint32_t)(key >> 32));
+      }
     }
   }
   if (m > k) __syncthreads();            // candidates that were not taken join the rest, in rank order
   if (tid < 64) {
-    double log_left = -INFINITY;
+    double hi = (double)ref * inv_t, sum_left = under;
     if (m > k) {
       const double top = (double)left[k] * inv_t;
-      double e = 0.0;
-      if (top == INFINITY) {
-        log_left = top;
-      } else if (!(top == -INFINITY)) {
-        for (int i = k + tid; i < m; i += 64) e += exp((double)left[i] * inv_t - top);
-        e = wave_reduce(e, SumOp());
-        log_left = top + log(e);
+      if (!(fabs(top - hi) <= 600.0)) {  // a reference of their own (or infinite, or NaN)
+        const double log_under = under > 0.0 ? hi + log(under) : -INFINITY;
+        sum_left = top == INFINITY || top == -INFINITY ? 0.0 : exp(log_under - top);
+        hi = top;
       }
+      double e = 0.0;
+      if (hi - hi == 0.0) {
+        for (int i = k + tid; i < m; i += 64) e += exp((double)left[i] * inv_t - hi);
+      }
+      sum_left += wave_reduce(e, SumOp());
     }
-    if (tid == 0) {
-      const double hi = log_left > log_under || log_left != log_left ? log_left : log_under;
-      const double lo = log_left > log_under || log_left != log_left ? log_under : log_left;
-      rest[n] = (float)(lo == -INFINITY ? hi : hi + log1p(exp(lo - hi)));
-    }
+    // an infinite or NaN `top` is the answer itself; the log of nothing is -inf
+    if (tid == 0) rest[n] = (float)(m > k && hi - hi != 0.0 ? hi : sum_left > 0.0 ? hi + log(sum_left) : sum_left != sum_left ? sum_left : -INFINITY);
   }
 }
 
@@ -408,7 +429,7 @@ struct DistillArgs {
 // LDS of a row's entries, behind them the bitmap of the vocabulary
 struct Entries {
   double p[TOPK_MAX];                    // teacher's logit over T, then exp(that - the largest)
-  float s[TOPK_MAX];                     // student's logit
+  double e[TOPK_MAX];                    // student's logit, then exp((that - the row's largest) / T)
   int32_t at[TOPK_MAX];                  // index, or -1
   double redd[4][16];
   double topd[16];
@@ -442,7 +463,7 @@ __device__ __forceinline__ double load_entries(const DistillArgs& a, int64_t n, 
     const double t = ok ? (double)load_scalar(a.values, e, a.vdt) * a.inv_t : -INFINITY;
     en.at[j] = ok ? (int32_t)at : -1;
     en.p[j] = t;
-    en.s[j] = ok ? load_scalar(row, at, DT) : -INFINITY;
+    en.e[j] = ok ? load_scalar(row, at, DT) : -INFINITY;
     if (ok && (atomicOr(&bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1)) en.dup = 1;
     mx = t > mx || t != t ? t : mx;      // NaN stays: it makes the row NaN, as in a softmax
   }
@@ -489,8 +510,8 @@ __device__ __forceinline__ void store_piece(void* row, int64_t at, const float (
 // The entries' gradients, over the zeros that the pass before them left there. The wait makes that pass's
 // stores complete (acknowledged by L2) before other waves of the workgroup store into the same lines.
 template <int DT, int NT>
-__device__ __forceinline__ void write_entries(const DistillArgs& a, int64_t n, Entries& en, float m_all, double inv_s,
-                                              double inv_total, float scale) {
+__device__ __forceinline__ void write_entries(const DistillArgs& a, int64_t n, Entries& en, double inv_s, double inv_total,
+                                              float scale) {
   char* out = (char*)a.grad + n * a.vocab * (DT == BCFFT_F32 ? 4 : 2);
   wait_vmcnt<0>();
   __syncthreads();
@@ -498,8 +519,7 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, int64_t n, E
     if (en.at[j] < 0) continue;
     double mass = en.p[j];
     if (!first_of(en, a.k, j, mass)) continue;
-    const double q = exp(((double)en.s[j] - (double)m_all) * a.inv_t) * inv_s;
-    store_one<DT>(out, en.at[j], (float)(q - mass * inv_total) * scale);
+    store_one<DT>(out, en.at[j], (float)(en.e[j] * inv_s - mass * inv_total) * scale);
   }
 }
 // The other elements': exp((v - ref) / T) times coef
@@ -581,18 +601,19 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
   double total = 0.0, se = 0.0, lin = 0.0;
   for (int j = tid; j < a.k; j += NT) {
     if (en.at[j] < 0) continue;
-    const double t = en.p[j] - am, p = exp(t), x = ((double)en.s[j] - (double)m_all) * a.inv_t;
+    const double t = en.p[j] - am, p = exp(t), x = (en.e[j] - (double)m_all) * a.inv_t, e = exp(x);
     en.p[j] = p;
+    en.e[j] = e;
     total += p;
     if (p > 0.0) lin += p * (t - x);
     else if (p != p) lin = p;
-    if (!en.dup) se += exp(x);
+    if (!en.dup) se += e;
   }
   if (en.dup) {                          // uniform: each index once
     __syncthreads();
     for (int j = tid; j < a.k; j += NT) {
       double mass;
-      if (en.at[j] >= 0 && first_of(en, a.k, j, mass)) se += exp(((double)en.s[j] - (double)m_all) * a.inv_t);
+      if (en.at[j] >= 0 && first_of(en, a.k, j, mass)) se += en.e[j];
     }
   }
   // the other elements' sum
@@ -669,13 +690,6 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
   // d loss / d s of an element outside the entries, over exp((v - ref) / T)
   const double shift = ref == m_all ? 1.0 : exp(((double)ref - (double)m_all) * a.inv_t);
   const double coef = shift * inv_s - (rest_p != 0.0 && sum_ref != 0.0 ? rest_p / sum_ref : 0.0);
-  if (tid == 0) {
-    // sum_j P_j ((a_j - am) - (s_j - m_all) / T) + log sum - log total, and the rest's part
-    double loss = sums[3] * inv_total + log(sum) + log(inv_total);
-    if (rest_p != 0.0) loss += rest_p * (rest_a - (((double)ref - (double)m_all) * a.inv_t + log(sum_ref)));
-    a.loss[n] = (float)loss * w;
-    if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * n) = make_float4(ref, (float)coef, m_all, (float)inv_s);
-  }
   if constexpr (GRAD) {
     const float scale = (float)(w * a.inv_t);
     if (KEEP && !again) {
@@ -702,7 +716,14 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
         write_others<DT>(a, n, r2, bits, ref, c);
       }
     }
-    write_entries<DT, NT>(a, n, en, m_all, inv_s, inv_total, scale);
+    write_entries<DT, NT>(a, n, en, inv_s, inv_total, scale);
+  }
+  if (tid == NT - 1) {                   // the last wave: the first ones write the entries meanwhile
+    // sum_j P_j ((a_j - am) - (s_j - m_all) / T) + log sum - log total, and the rest's part
+    double loss = sums[3] * inv_total + log(sum) + log(inv_total);
+    if (rest_p != 0.0) loss += rest_p * (rest_a - (((double)ref - (double)m_all) * a.inv_t + log(sum_ref)));
+    a.loss[n] = (float)loss * w;
+    if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * n) = make_float4(ref, (float)coef, m_all, (float)inv_s);
   }
 }
 
@@ -721,19 +742,20 @@ __global__ __launch_bounds__(NT) void bc_distill_backward_kernel(DistillArgs a) 
     write_zero<DT, NT>(a, n);
     return;
   }
+  const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * n);
   double total = 0.0;
   for (int j = threadIdx.x; j < a.k; j += NT) {
     if (en.at[j] < 0) continue;
     en.p[j] = exp(en.p[j] - am);
+    en.e[j] = exp((en.e[j] - (double)st.z) * a.inv_t);
     total += en.p[j];
   }
   total = block_reduce<NT>(total, en.topd, SumOp()) + (a.rest ? exp((double)a.rest[n] - am) : 0.0);
-  const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * n);
   const float scale = (float)(w * a.inv_t) * a.upstream[n];
   Row<DT, NT, 0> r;
   r.open(row, a.vocab);
   write_others<DT>(a, n, r, bits, st.x, st.y * scale);
-  write_entries<DT, NT>(a, n, en, st.z, st.w, 1.0 / total, scale);
+  write_entries<DT, NT>(a, n, en, st.w, 1.0 / total, scale);
 }
 
 // ------------------------------------------------------------------ launches
