@@ -133,11 +133,47 @@ struct Row {
 template <class A> constexpr int count_of = (int)(sizeof(std::remove_reference_t<A>) / sizeof(float));
 
 // ------------------------------------------------------------------ reductions over the workgroup
+// Lanes trade values inside the vector unit: by shuffles through LDS a sum of doubles over the workgroup takes
+// 1600 clocks, so 500. Steps 1, 2: neighbours in groups of 4; 4, 8: a mirror image of 8, 16 lanes, whose halves
+// each hold one value by then.
+template <int STEP>
+__device__ __forceinline__ uint32_t other_lane(uint32_t v) {
+  constexpr int CTRL = STEP == 1 ? 0xb1 : STEP == 2 ? 0x4e : STEP == 4 ? 0x141 : 0x140;
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int STEP, class T>
+__device__ __forceinline__ T other(T v) {
+  if constexpr (sizeof(T) == 8) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(T, (uint64_t)other_lane<STEP>((uint32_t)(b >> 32)) << 32 | other_lane<STEP>((uint32_t)b));
+  } else {
+    return __builtin_bit_cast(T, other_lane<STEP>(__builtin_bit_cast(uint32_t, v)));
+  }
+}
+// over LANES <= 16 neighbouring lanes
+template <int LANES, class T, class OP>
+__device__ __forceinline__ T lanes_reduce(T v, OP op) {
+  if constexpr (LANES > 1) v = op(v, other<1>(v));
+  if constexpr (LANES > 2) v = op(v, other<2>(v));
+  if constexpr (LANES > 4) v = op(v, other<4>(v));
+  if constexpr (LANES > 8) v = op(v, other<8>(v));
+  return v;
+}
 template <class T, class OP>
 __device__ __forceinline__ T wave_reduce(T v, OP op) {
+  v = lanes_reduce<16>(v, op);
+  T w[4];                                // the four groups' results, the same in every lane
 #pragma unroll
-  for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
-  return v;
+  for (int g = 0; g < 4; ++g) {
+    if constexpr (sizeof(T) == 8) {
+      const uint64_t b = __builtin_bit_cast(uint64_t, v);
+      w[g] = __builtin_bit_cast(T, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 16 * g) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 16 * g));
+    } else {
+      w[g] = __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 16 * g));
+    }
+  }
+  return op(op(w[0], w[1]), op(w[2], w[3]));
 }
 struct MaxOp {
   // a NaN on either side stays
@@ -150,10 +186,7 @@ struct SumOp {
 // loop over them would hold all)
 template <int NT, class T, class OP>
 __device__ __forceinline__ T across_waves(const T* red, OP op) {
-  T v = red[threadIdx.x & (NT / 64 - 1)];
-#pragma unroll
-  for (int d = NT / 128; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
-  return v;
+  return lanes_reduce<NT / 64>(red[threadIdx.x & (NT / 64 - 1)], op);
 }
 // every thread gets the result, added up in a fixed order; `red` holds NT / 64 values and is free
 // again after the caller's next barrier
@@ -226,8 +259,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
   uint32_t key = any ? order_key(best) : 0;
   const bool grouped = NT > 256 && k <= 128;
   if (grouped) {
-#pragma unroll
-    for (int d = 1; d < NT / 256; d *= 2) key = max(key, (uint32_t)__shfl_xor((int)key, d, 64));
+    key = lanes_reduce<NT / 256>(key, MaxOp());
     if (tid % (NT / 256) == 0) gmax[tid / (NT / 256)] = key;
   } else {
     gmax[tid] = key;
@@ -376,8 +408,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
     int rank = 0;
 #pragma unroll 4
     for (int j = tid % 16; j < m; j += 16) rank += cand[j] > key;
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) rank += __shfl_xor(rank, d, 64);
+    rank = lanes_reduce<16>(rank, SumOp());
     if (i < m && tid % 16 == 0) {
       if (rank < k) {
         if constexpr (DT == BCFFT_F32) ((uint32_t*)values)[n * k + rank] = raw[i];
