@@ -812,17 +812,45 @@ static void by_row(int64_t vocab, int64_t min_threads, F&& go) {
   else go(integral_constant<int, 1024>(), integral_constant<int, 0>());
 }
 
-template <int DT>
-static void launch_topk_dt(const void* logits, int64_t n, int64_t vocab, int64_t row_stride, int k, double temperature,
-                           void* values, int32_t* indices, float* rest, hipStream_t s) {
-  by_row<DT>(vocab, k, [&](auto nt, auto hold) {
-    hipLaunchKernelGGL((bc_topk_logits_kernel<DT, nt.value, hold.value>), dim3((unsigned)n), dim3(nt.value), 0, s,
-                       logits, vocab, row_stride, k, exp_scale(temperature), 1.0 / temperature, values, indices, rest);
-  });
+// A launch holds fewer than 2^32 threads: rows by the 2^21 (of up to 1024 threads each)
+constexpr int64_t LAUNCH_ROWS = 1 << 21;
+template <class F>
+static void by_rows(int64_t n, F&& go) {
+  for (int64_t first = 0; first < n; first += LAUNCH_ROWS) go(first, n - first < LAUNCH_ROWS ? n - first : LAUNCH_ROWS);
 }
 
 template <int DT>
-static void launch_distill_dt(const DistillArgs& a, int64_t n, hipStream_t s) {
+static void launch_topk_dt(const void* logits, int64_t n, int64_t vocab, int64_t row_stride, int k, double temperature,
+                           void* values, int32_t* indices, float* rest, hipStream_t s) {
+  constexpr int64_t E = DT == BCFFT_F32 ? 4 : 2;
+  by_row<DT>(vocab, k, [&](auto nt, auto hold) {
+    by_rows(n, [&](int64_t at, int64_t rows) {
+      hipLaunchKernelGGL((bc_topk_logits_kernel<DT, nt.value, hold.value>), dim3((unsigned)rows), dim3(nt.value), 0, s,
+                         (const char*)logits + at * row_stride * E, vocab, row_stride, k, exp_scale(temperature),
+                         1.0 / temperature, (char*)values + at * k * E, indices + at * k, rest + at);
+    });
+  });
+}
+
+// the operands from row `at` on
+template <int DT>
+static DistillArgs from_row(const DistillArgs& a, int64_t at) {
+  constexpr int64_t E = DT == BCFFT_F32 ? 4 : 2;
+  auto plus = [&](auto* p, int64_t by) { return p ? p + by : nullptr; };
+  DistillArgs b = a;
+  b.logits = (const char*)a.logits + at * a.row_stride * E;
+  b.values = (const char*)a.values + at * a.k * (a.vdt == BCFFT_F32 ? 4 : 2);
+  b.indices = (const char*)a.indices + at * a.k * (a.idx64 ? 8 : 4);
+  b.rest = plus(a.rest, at);
+  b.weight = plus(a.weight, at);
+  b.upstream = plus(a.upstream, at);
+  b.loss = plus(a.loss, at);
+  b.stats = plus(a.stats, 4 * at);
+  b.grad = plus((char*)a.grad, at * a.vocab * E);
+  return b;
+}
+template <int DT>
+static void launch_distill_rows(const DistillArgs& a, int64_t n, hipStream_t s) {
   const unsigned lds = (unsigned)((a.vocab + 31) / 32 * 4);
   if (a.upstream) {
     hipLaunchKernelGGL((bc_distill_backward_kernel<DT, 512>), dim3((unsigned)n), dim3(512), lds, s, a);
@@ -832,6 +860,10 @@ static void launch_distill_dt(const DistillArgs& a, int64_t n, hipStream_t s) {
     if (a.grad) hipLaunchKernelGGL((bc_distill_kernel<DT, nt.value, hold.value, true>), dim3((unsigned)n), dim3(nt.value), lds, s, a);
     else hipLaunchKernelGGL((bc_distill_kernel<DT, nt.value, hold.value, false>), dim3((unsigned)n), dim3(nt.value), lds, s, a);
   });
+}
+template <int DT>
+static void launch_distill_dt(const DistillArgs& a, int64_t n, hipStream_t s) {
+  by_rows(n, [&](int64_t at, int64_t rows) { launch_distill_rows<DT>(from_row<DT>(a, at), rows, s); });
 }
 static int launch_distill(int dt, const DistillArgs& a, int64_t n, hipStream_t s) {
   if (dt == BCFFT_F32) launch_distill_dt<BCFFT_F32>(a, n, s);

@@ -452,3 +452,58 @@ def test_extreme_temperatures(dev):
         at, r = teacher_oracle(s, 9, t)
         assert torch.equal(i2.cpu().long(), at)
         assert bool(((rest.double().cpu() - r).abs() <= LOG_TOL + 2.0 ** -22 * r.abs()).all())
+
+
+def test_offsets_past_32_bits(dev):
+    """Logits and gradients of 9000 x 262144 (2.4e9 elements): what the last rows hold."""
+    from bcfft import distill
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB of device memory")
+    n, v, k = 9000, 1 << 18, 7
+    z = torch.randn(n, v, generator=torch.Generator(device=dev).manual_seed(51), device=dev, dtype=torch.float16)
+    values, indices, rest = distill.topk_logits(z, k, 2.0)
+    rows = [0, n - 2, n - 1]
+    top, want = teacher_oracle(z[rows], k, 2.0)
+    assert torch.equal(indices[rows].cpu().long(), top)
+    assert bool(((rest[rows].double().cpu() - want).abs() <= LOG_TOL + 2.0 ** -23 * want.abs()).all())
+    shifted = indices.roll(1, 0)                          # another row's entries: q and P differ
+    loss, grad = distill.topk_kl_grad(z, values, shifted, rest=rest, temperature=2.0)
+    lk, dk, size = kl_oracle(z[rows], values[rows], shifted[rows], rest[rows], None, 2.0)
+    check_loss(loss[rows], lk)
+    check_grad(grad[rows], dk, size)
+    zg = z.requires_grad_()
+    distill.topk_kl(zg, values, shifted, rest=rest, temperature=2.0).sum().backward()
+    check_grad(zg.grad[rows], dk, size)
+
+
+def test_more_rows_than_one_launch(dev):
+    """2^21 + 5 rows: rows behind the first launch's find their own operands."""
+    from bcfft import distill
+    n, v, k, t = (1 << 21) + 5, 9, 3, 1.5
+    g = torch.Generator(device=dev).manual_seed(52)
+    z = torch.randn(n, v, generator=g, device=dev).to(torch.float16)
+    weight = torch.rand(n, generator=g, device=dev)
+    values, indices, rest = distill.topk_logits(z, k, t)
+    z64 = z.double()
+    keys = z64 * 64 - torch.arange(v, device=dev) * 2.0 ** -20      # equal logits: lower index first
+    top = keys.topk(k, dim=-1).indices
+    assert torch.equal(indices.long(), top) and torch.equal(values, z.gather(-1, top))
+    left = torch.ones_like(z64).scatter_(-1, top, 0.0).bool()
+    r64 = torch.logsumexp((z64 / t).masked_fill(~left, NEG), -1)
+    assert bool(((rest.double() - r64).abs() <= LOG_TOL + 2.0 ** -23 * r64.abs()).all())
+    s = torch.randn(n, v, generator=g, device=dev)
+    logq = torch.log_softmax(s.double() / t, -1)
+    logp = torch.log_softmax(torch.cat([values.double() / t, rest.double()[:, None]], -1), -1)
+    log_rest = torch.logsumexp(logq.masked_fill(~left, NEG), -1)
+    p, q = logp.exp(), logq.exp()
+    want = ((p[:, :k] * (logp[:, :k] - logq.gather(-1, top))).sum(-1) + p[:, k] * (logp[:, k] - log_rest)) * weight.double()
+    share = torch.where(left, p[:, k:] * torch.exp(logq - log_rest[:, None]), 0.0).scatter_(-1, top, p[:, :k])
+    f = weight.double()[:, None] / t
+    dwant, size = ((q - share) * f).cpu(), ((q + share) * f).cpu()
+    loss, grad = distill.topk_kl_grad(s, values, indices, rest=rest, weight=weight, temperature=t)
+    check_loss(loss, want.cpu(), weight)
+    check_grad(grad, dwant, size)
+    sg = s.clone().requires_grad_()
+    loss = distill.topk_kl(sg, values, indices.long(), rest=rest, weight=weight, temperature=t)
+    loss.backward(torch.full_like(loss, 3.0))
+    check_grad(sg.grad, dwant, size, 3.0)
