@@ -9,7 +9,9 @@ operators, differentiable in every operand:
 
 patch_llama_fft.fuse_dense_mlp routes the dense MLPs of a model through them. Every function enqueues on the
 current stream of x's device and does not synchronise. There is no CPU path: a host tensor raises
-RuntimeError.
+RuntimeError. To capture a training step into a graph, capture forward and backward together, with no eager
+graph of the same parameters alive. A call that records a gradient runs eagerly (under torch.compile, in a
+torch.compiler.disable region); torch.ops.bcfft.dense_linear / dense_glu carry the forward through a trace.
 """
 from __future__ import annotations
 

@@ -55,6 +55,13 @@ int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.siz
 Tensor aligned16(const Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone(at::MemoryFormat::Contiguous) : t;
 }
+// FakeTensors and functionalised tensors have no memory: their shapes come from the Meta kernels, but a C++
+// autograd node here would read them
+void require_memory(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python), what,
+              ": records no gradient of a traced tensor (FakeTensor, torch.compile); run this call eagerly, e.g. under "
+              "torch.compiler.disable");
+}
 // as torch.autograd.function.once_differentiable: a second differentiation raises instead of missing terms
 variable_list once(variable_list out, const Tensor& upstream) {
   if (!(at::GradMode::is_enabled() && wants_grad(upstream))) return out;
@@ -419,23 +426,30 @@ auto below(const char* name, F) {
 Tensor dense_linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t act) {
   if (at::GradMode::is_enabled() && !x.is_meta()) {
     const bool inner = wants_grad(x) || wants_grad(weight) || wants_grad(bias);
-    if (inner || wants_grad(residual)) return LinearFn::apply(x, weight, bias, residual, act, inner && act != BCFFT_ACT_NONE);
+    if (inner || wants_grad(residual)) {
+      require_memory(x, LINEAR);
+      return LinearFn::apply(x, weight, bias, residual, act, inner && act != BCFFT_ACT_NONE);
+    }
   }
   at::AutoDispatchBelowADInplaceOrView guard;
   static auto op = below("bcfft_native::dense_linear", &dense_linear_hip);
   return op.call(x, weight, bias, residual, act);
 }
 Tensor dense_glu_autograd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int64_t act) {
-  if (at::GradMode::is_enabled() && !x.is_meta() && (wants_grad(x) || wants_grad(w_gate) || wants_grad(w_up)))
+  if (at::GradMode::is_enabled() && !x.is_meta() && (wants_grad(x) || wants_grad(w_gate) || wants_grad(w_up))) {
+    require_memory(x, GLU);
     return GluFn::apply(x, w_gate, w_up, act);
+  }
   at::AutoDispatchBelowADInplaceOrView guard;
   static auto op = below("bcfft_native::dense_glu", &dense_glu_hip);
   return op.call(x, w_gate, w_up, act);
 }
 Tensor topk_kl_autograd(const Tensor& logits, const Tensor& values, const Tensor& indices, const OptTensor& rest,
                         const OptTensor& weight, double temperature) {
-  if (at::GradMode::is_enabled() && !logits.is_meta() && wants_grad(logits))
+  if (at::GradMode::is_enabled() && !logits.is_meta() && wants_grad(logits)) {
+    require_memory(logits, KL);
     return TopKKlFn::apply(logits, values, indices, rest, weight, temperature);
+  }
   at::AutoDispatchBelowADInplaceOrView guard;
   static auto op = below("bcfft_native::topk_kl", &topk_kl_hip);
   return op.call(logits, values, indices, rest, weight, temperature);

@@ -84,3 +84,37 @@ def test_host_tensors_are_refused(built_lib):
             dense.linear(x.clone().requires_grad_(grad), w)
         with pytest.raises(RuntimeError, match="ROCm device"):
             dense.glu(x.clone().requires_grad_(grad), w, w)
+
+
+def test_fake_shapes(built_lib):
+    """FakeTensors: the registered operators give shapes and dtypes without a device or a launch."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from bcfft import _lib, dense, torch_ops  # noqa: F401
+    with FakeTensorMode():
+        for dt in (torch.float32, torch.bfloat16):
+            x, w = torch.empty(2, 5, 64, device="cuda", dtype=dt), torch.empty(48, 64, device="cuda", dtype=dt)
+            y = torch.ops.bcfft.dense_linear(x, w, None, None, "gelu")
+            h = torch.ops.bcfft.dense_glu(x, w, w, "silu")
+            for t in (y, h):
+                assert t.shape == (2, 5, 48) and t.dtype == dt and t.device.type == "cuda"
+            if _lib.native_op():
+                assert dense.linear(x, w).shape == dense.glu(x, w, w).shape == (2, 5, 48)
+        with pytest.raises(ValueError, match="in_features"):
+            torch.ops.bcfft.dense_linear(x, w.t(), None, None, "none")
+        with pytest.raises(ValueError, match="in_features"):
+            torch.ops.bcfft.dense_glu(x, w, w[:3], "silu")
+
+
+def test_traced_gradients_are_refused(built_lib):
+    """A C++ autograd node would read memory that a FakeTensor does not have."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from bcfft import _lib, dense, distill
+    if not _lib.native_op():
+        pytest.skip("the C++ operators are not built")
+    with FakeTensorMode():
+        x = torch.empty(4, 64, device="cuda", requires_grad=True)
+        w = torch.empty(48, 64, device="cuda")
+        for call in (lambda: dense.linear(x, w), lambda: dense.glu(x, w, w),
+                     lambda: distill.topk_kl(x, w[:4, :3], torch.empty(4, 3, device="cuda", dtype=torch.int32))):
+            with pytest.raises(RuntimeError, match="traced"):
+                call()
