@@ -459,9 +459,13 @@ def fuse_mlp_gate_up(model) -> int:
 
 
 def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
-    """The dense kernels take device tensors of one dtype; anything else runs the modules' own forward."""
+    """The dense kernels take device tensors of one dtype and plain nn.Linear modules; anything else (autocast,
+    a projection replaced later, hooks on one) runs the modules' own forward."""
+    for m in (mlp.gate_proj, mlp.up_proj, mlp.down_proj):
+        if type(m) is not nn.Linear or m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
+            return False
     ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
-    return (x.is_cuda and x.dtype in _lib.DTYPE_CODE and not torch.is_autocast_enabled("cuda")
+    return (mlp.gate_proj.bias is None and mlp.up_proj.bias is None and x.is_cuda and x.dtype in _lib.DTYPE_CODE and not torch.is_autocast_enabled("cuda")
             and all(t is None or (t.dtype == x.dtype and t.device == x.device) for t in ws))
 
 
@@ -479,8 +483,9 @@ def fuse_dense_mlp(model) -> int:
     31 of 32 layers with the reference's default NUM_LAYERS_TO_PATCH) through the dense kernels: the gate and
     up projections with their product in one launch, the down projection in another, in training too
     (bcfft.dense is differentiable in every operand). The rewired forward also takes a residual that the
-    down projection adds in its epilogue. Parameters and state_dict are unchanged; replacing one of the
-    three modules afterwards needs a new call. Returns the number of MLPs rewired."""
+    down projection adds in its epilogue. Parameters and state_dict are unchanged; an MLP one of whose three
+    modules is replaced afterwards or holds hooks runs the modules' own forward. Returns the number of MLPs
+    rewired."""
     import types
     n = 0
     for layer in model.model.layers:

@@ -79,8 +79,8 @@ def test_calibration_step(dev):
 
 def test_fused_dense_mlp_forward(dev):
     """bf16, no gradient: prefill and single tokens, with and without the residual, against the modules in fp64.
-    h is rounded once to bf16 (2^-9 at most, half a step) and y once: 2 * 2^-9 in the norm, and the inner sums'
-    2^-20 beside it."""
+    h is rounded once to bf16 (2^-8 at most, half a step) and y once: below 2 * 2^-8 in the norm, the inner
+    sums' 2^-20 included."""
     import patch_llama_fft as P
     _, student = build(dev, torch.bfloat16)
     P.fuse_dense_mlp(student)
@@ -118,3 +118,25 @@ def test_fused_dense_mlp_other_inputs(dev):
         assert P.fuse_dense_mlp(teacher) == 3
         y = teacher.model.layers[0].mlp(torch.randn(2, 3, 256, device=dev))
     assert y.dtype == torch.bfloat16                   # autocast's own products
+
+
+def test_fused_dense_mlp_hooks_and_replaced_modules(dev):
+    """A projection with a hook, or replaced after the call, is called as the module it is."""
+    import patch_llama_fft as P
+    teacher, _ = build(dev)
+    assert P.fuse_dense_mlp(teacher) == 3
+    mlp = teacher.model.layers[0].mlp
+    x = torch.randn(2, 3, 256, device=dev)
+    with torch.no_grad():
+        want = mlp(x)
+    seen = []
+    hook = mlp.up_proj.register_forward_hook(lambda m, i, o: seen.append(o.shape))
+    y = mlp(x).detach()
+    assert seen == [(2, 3, 512)]
+    assert float((y - want).norm() / want.norm()) < 1e-4
+    hook.remove()
+    assert torch.equal(mlp(x).detach(), want) and len(seen) == 1
+    mlp.down_proj = torch.nn.Sequential(mlp.down_proj, torch.nn.Tanh())
+    assert float((mlp(x).detach() - want.tanh()).abs().max()) < 1e-4
+    mlp.gate_proj = torch.nn.Linear(256, 512, bias=True).to(dev)
+    assert mlp(x).shape == x.shape
