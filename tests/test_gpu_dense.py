@@ -403,3 +403,86 @@ def test_second_derivative_is_refused(dev):
         (dx,) = torch.autograd.grad(y, x, up, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiate twice"):
             dx.sum().backward()
+
+
+def test_offsets_past_32_bits(dev):
+    """Rows of x that lie 2^20 elements apart (2.2e9 in all), and outputs, saved inputs and gradients of
+    70000 x 32000 (2.2e9): what the last ones hold."""
+    from bcfft import dense
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 90 GB of device memory")
+    dt = torch.bfloat16
+    wide = torch.empty(2100, 1 << 20, dtype=dt, device=dev)
+    wide[:, :64] = rand(dev, 2100, 64, dt=dt, seed=91)
+    x, w = wide[:, :64], rand(dev, 40, 64, dt=dt, seed=92, scale=0.125)
+    assert torch.equal(dense.linear(x, w), dense.linear(x.contiguous(), w))
+    dy = rand(dev, 2100, 40, dt=dt, seed=93)
+    xg, wg = x.detach().requires_grad_(), w.clone().requires_grad_()
+    dense.linear(xg, wg, activation="silu").backward(dy)
+    xc, wc = x.detach().contiguous().requires_grad_(), w.clone().requires_grad_()
+    dense.linear(xc, wc, activation="silu").backward(dy)
+    assert torch.equal(wg.grad, wc.grad) and torch.equal(xg.grad, xc.grad)
+    del wide, x, xg
+
+    n, k, m = 70000, 32, 32000
+    x, w, wu = (rand(dev, *s, dt=dt, seed=94 + i, scale=0.2) for i, s in enumerate(((n, k), (m, k), (m, k))))
+    b, r = rand(dev, m, dt=dt, seed=97), rand(dev, n, m, dt=dt, seed=98)
+    y = dense.linear(x, w, b, activation="gelu", residual=r)
+    rows = slice(n - 300, n)
+    want, slack, *_ = linear64(x[rows], w, b, r[rows], "gelu")
+    within(y[rows], want, slack)
+    del y, want, slack
+    ins = [t.clone().requires_grad_() for t in (x, w, wu)]
+    h = dense.glu(*ins)
+    g64, u64 = x[rows].double() @ w.double().t(), x[rows].double() @ wu.double().t()
+    v, slope = act64(g64, "silu")
+    gs, us = sum_slack(x[rows].double(), w.double().t()), sum_slack(x[rows].double(), wu.double().t())
+    within(h[rows], v * u64, (1.2 * gs + 16 * U * v.abs()) * u64.abs() + v.abs() * us + U * (v * u64).abs())
+    h.backward(r)                                         # r in dh's place
+    d = r[rows].double()
+    eps = torch.finfo(dt).eps / 2
+    w64, wu64 = w.double(), wu.double()
+    dg, du = d * u64 * slope, d * v
+    dx = dg @ w64 + du @ wu64
+    mag = sum_slack(torch.cat([dg, du], 1), torch.cat([w64, wu64], 0))
+    rounding = 8 * eps * torch.sqrt((dg * dg) @ (w64 * w64) + (du * du) @ (wu64 * wu64))
+    inner = (d.abs() * (us * slope.abs() + u64.abs() * (1.2 * gs + 16 * U))) @ w64.abs() + \
+            (d.abs() * (1.2 * gs + 16 * U * v.abs())) @ wu64.abs()
+    within(ins[0].grad[rows], dx, mag + rounding + inner)
+    del dg, du, d, g64, u64, v, slope, gs, us, mag, rounding, inner
+    cols = slice(m - 40, m)                               # the last output features' weight gradients
+    x64, d = x.double(), r[:, cols].double()
+    g64, u64 = x64 @ w64[cols].t(), x64 @ wu64[cols].t()
+    v, slope = act64(g64, "silu")
+    gs, us = sum_slack(x64, w64[cols].t()), sum_slack(x64, wu64[cols].t())
+    dg, du = d * u64 * slope, d * v
+    for got, dz, err in ((ins[1].grad, dg, d.abs() * (us * slope.abs() + u64.abs() * (1.2 * gs + 16 * U))),
+                         (ins[2].grad, du, d.abs() * (1.2 * gs + 16 * U * v.abs()))):
+        want = dz.t() @ x64
+        slack = sum_slack(dz.t(), x64) + err.t() @ x64.abs() + 8 * eps * torch.sqrt((dz * dz).t() @ (x64 * x64))
+        within(got[cols], want, slack)
+
+
+def test_two_streams_at_once(dev):
+    """Calls that overlap on two streams share nothing: each has its own workspace (split k, dz, packed rows)."""
+    from bcfft import dense
+    args = [[rand(dev, *s, dt=torch.float16, seed=101 + 7 * i + j, scale=0.1)
+             for j, s in enumerate(((70, 2001), (130, 2001), (130, 2001), (70, 130)))] for i in range(2)]
+
+    def step(x, w, wu, dh):
+        ins = [t.detach().clone().requires_grad_() for t in (x, w, wu)]
+        h = dense.glu(*ins, activation="gelu") + dense.linear(ins[0], ins[1], activation="silu")
+        return (h.detach(),) + torch.autograd.grad(h, ins, dh)
+
+    want = [step(*a) for a in args]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
