@@ -116,15 +116,19 @@ __global__ __launch_bounds__(256) void bc_dense_pack_kernel(const char* __restri
 
 // ------------------------------------------------------------------ launches
 // Tile and slices for an m x n product over ksteps tiles of k, with `parts` products per output (2: gated):
-// the least estimated time in microseconds. step: one tile of k of one workgroup with its CU's share, fixed: its
-// start and its outputs (16-bit: measured at 8192 x 4096 x 4096, 2048 x 4096 x 64 to 4096 and, by columns,
-// 22016 x 4096 x 1700; fp32: the fp32 matrix rate). cols: operands that lie by columns (256 x 128 tiles read
-// theirs in rows of 256 bytes). Slices pay their partial sums' way through memory and the finishing launch.
+// the least estimated time in microseconds. A CU's time for one tile of k of one workgroup is idle + busy u, u
+// the part of the chip's slots that is taken over the call (the clock and the caches give way under load:
+// 256 x 256 tiles 1.06 us at u = 0.44, 1.30 at 0.78, 1.45 at 1); fixed: a workgroup's start and its outputs.
+// 16-bit values fitted to 4096 x 4096 x 4096, 8192 x 4096 x 4096, 1700 x 4096 x 11008, 1700 x 2 (11008) x 4096 and
+// 2048 x 4096 x 64, fp32 to 2048 x 4096 x 64 and 1024, 4096 x 4096 x 1024 and 5963 x 6240 x 128: all within 5 %
+// (k = 64 aside). cols: operands that lie by columns, 0.06 us each. Slices pay their partial sums' way through
+// memory and the finishing launch (1700 x 4096 x 22016 in two: 262 + 13 us, whole 301).
 static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int cols) {
   if (cols == 0 && m <= 32) return {0, 1};
   const int64_t cus = device_cu_count();
-  struct Kind { int kind, bm, bn, slots; double step, step32, fixed; };
-  const Kind kinds[3] = {{1, 128, 128, 2, 0.48, 1.9, 2.5}, {2, 256, 128, 1, 0.82 + 0.06 * cols, 3.7, 3.0}, {3, 256, 256, 1, 1.55, 7.3, 6.0}};
+  struct Kind { int kind, bm, bn; double idle, busy, fixed, step32, fixed32; };
+  const Kind kinds[3] = {{1, 128, 128, 0.46, 0.0, 2.5, 1.85, 4.5}, {2, 256, 128, 0.35, 0.49, 3.0, 3.72, 9.6},
+                         {3, 256, 256, 0.75, 0.70, 6.0, 7.3, 16.0}};
   Shape best{1, 1};
   double least = 1e300;
   for (const Kind& q : kinds) {
@@ -132,9 +136,11 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
     for (int64_t kz = 1; kz <= 16 && (kz == 1 || ksteps / kz >= 4); ++kz) {
       const int64_t groups = tiles * kz;
       const int64_t per_cu = (groups + cus - 1) / cus;                   // the fullest CU's workgroups
-      const double step = dt == BCFFT_F32 ? q.step32 : q.step * (q.slots == 2 && per_cu == 1 ? 1.3 : 1.0);
-      double cost = (double)per_cu * ((double)((ksteps + kz - 1) / kz) * step + q.fixed);
-      if (kz > 1) cost += 4.0 + (double)(2 * kz) * m * n * parts * 4.0 / 4e6;
+      const double used = (double)groups / (double)(per_cu * cus);
+      double step = dt == BCFFT_F32 ? q.step32 : q.idle + q.busy * used + 0.06 * cols;
+      if (q.kind == 1 && per_cu == 1) step *= dt == BCFFT_F32 ? 1.15 : 1.3;    // two of these share a CU's gaps
+      double cost = (double)per_cu * ((double)((ksteps + kz - 1) / kz) * step + (dt == BCFFT_F32 ? q.fixed32 : q.fixed));
+      if (kz > 1) cost += 4.0 + (double)(2 * kz) * m * n * parts * 4.0 / 5e6;
       if (cost < least) {
         least = cost;
         best = {q.kind, (int)kz};

@@ -149,12 +149,18 @@ template <int N>
 __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+// this wave's LDS reads complete, then the rendezvous
+__device__ __forceinline__ void tile_reuse() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // ------------------------------------------------------------------ the tile kernel
 // WM x WN waves, each (BM / WM) x (BN / WN) of the BM x BN tile in accumulators. A tile of k is 2 FM steps,
 // one row fragment against all column fragments each. What keeps the matrix cores fed:
-//  - RA LDS buffers of A and RB of B (256 x 256: 3 and 2, all 160 KB), so that loads are in flight at every
-//    moment: with 2 and 2 the stream stops at each barrier (8192 x 4096 x 4096 bf16: 1188 -> 1321 TFLOP/s).
+//  - Two tiles of k are in flight behind the one that is read, at every moment (8192 x 4096 x 4096 bf16: 1188
+//    TFLOP/s with one). 256 x 128 tiles have three LDS buffers of A and of B. 256 x 256 tiles fill the 160 KB
+//    with three of A and two of B (RB = 2): B's second fragments are in registers before half of a tile's
+//    steps are done, a barrier there (HALF) frees its buffer, and the tile after the next goes into it
+//    (operands from HBM: 1257 -> 1367 TFLOP/s against loads that wait for the end of the tile; 8192 x 2 (11008) x
+//    4096, gated: 1150 -> 1053 us).
 //  - The loads of later tiles are issued one per step or two. In one burst after the barrier they hold all
 //    waves at the address unit.
 //  - k tiles of 128 bytes: 64-byte pieces of rows fetch every 128-byte cache line twice (1101 -> 1025
@@ -164,8 +170,8 @@ __device__ __forceinline__ void tile_barrier() {
 //    next tile run under the last products of this one.
 //  - No branch in the loop: past a run's end the last tile is loaded again and never read.
 // 8 waves: with 4 of twice the size the single wave of a SIMD leaves its gaps open (1321 -> 1043).
-// MFMA busy 51 % -> 58 % of the cycles; the rest is the waves' meeting at the barriers and, past that, the
-// clock under load (2.2 GHz of 2.4).
+// Matrix cores busy (gated 8192 x 2 (11008) x 4096): 61 % of the cycles with loads that wait, 74 % so; the clock
+// under that load falls from 2.0 to 1.8 GHz, which is what bounds it now.
 // GLU: B's tile is BN / 2 rows of the gate weight and BN / 2 of the up weight, and a wave holds the same
 // columns of both, so the product of the two needs no exchange.
 // Both operands' rows start on 16 bytes (by columns: and hold a multiple of 16 bytes).
@@ -179,7 +185,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void bc_dense_tile_kernel(DenseArg
   using OB = Operand<DT, BR, CB, NT>;
   constexpr int LA = OA::PER, LB = NB * OB::PER;       // loads per thread and tile
   static_assert(!GLU || !CB, "the gated form reads weights by rows");
-  static_assert((RA == RB || RA == RB + 1) && RB >= 2, "the order of the loads in flight");
+  constexpr bool REUSE = RB == 2;
+  static_assert(RA == 3 && (RB == 3 || RB == 2), "two tiles in flight behind the one that is read");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave / WN, wn = wave % WN;
@@ -216,7 +223,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void bc_dense_tile_kernel(DenseArg
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int STEPS = 2 * FM;
+  constexpr int STEPS = 2 * FM, HALF = FN + (FM > FN ? 2 : 0);
+  static_assert(FN <= FM && HALF < STEPS - 2, "B's second half is read before its buffer is loaded anew");
   uint4 va[4], vb[2][FN];
   auto read_a = [&](const char* tile, int s) { return fa.read(tile, wm * TM + s % FM * 16, s / FM); };
   auto read_b = [&](const char* tile, int j, int kk) {
@@ -269,17 +277,15 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void bc_dense_tile_kernel(DenseArg
         wb = wb + BBYTES == RA * ABYTES + RB * BBYTES ? RA * ABYTES : wb + BBYTES;
       };
 #pragma unroll
-      for (int p = 0; p < RA - 1; ++p) {
+      for (int p = 0; p < 2; ++p) {
 #pragma unroll
         for (int i = 0; i < LA; ++i) load_a(i);
         next_a();
-        if (p < RB - 1) {
 #pragma unroll
-          for (int i = 0; i < LB; ++i) load_b(i);
-          next_b();
-        }
+        for (int i = 0; i < LB; ++i) load_b(i);
+        next_b();
       }
-      constexpr int YOUNG = (RA - 2) * LA + (RB - 2) * LB;   // loads of tiles after the next one
+      constexpr int YOUNG = LA + LB;                   // loads of the tile after the next one
       tile_barrier<YOUNG>();
       first_reads(lds, lds_b);
       for (int t = 0; t < run; ++t) {
@@ -287,21 +293,19 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void bc_dense_tile_kernel(DenseArg
         const char* tb = lds_b + rb;
         ra = ra + ABYTES == RA * ABYTES ? 0 : ra + ABYTES;
         rb = rb + BBYTES == RB * BBYTES ? 0 : rb + BBYTES;
-        constexpr int ISSUE = STEPS - 2;
+        constexpr int ISSUE = STEPS - 2, FIRST = REUSE ? HALF : ISSUE * LA / (LA + LB);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
           const int kk = s / FM, i = s % FM;
+          if (REUSE && s == HALF) tile_reuse();        // every wave holds B's fragments
           if (s + 2 < STEPS) va[(s + 2) % 4] = read_a(ta, s + 2);
-          if (kk == 0) {
+          if (s < FN) vb[1][s] = read_b(tb, s, 1);
+          if (s < FIRST) {
 #pragma unroll
-            for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j) vb[1][j] = read_b(tb, j, 1);
-          }
-          if (s < ISSUE) {
+            for (int q = s * LA / FIRST; q < (s + 1) * LA / FIRST; ++q) load_a(q);
+          } else if (s < ISSUE) {
 #pragma unroll
-            for (int q = s * (LA + LB) / ISSUE; q < (s + 1) * (LA + LB) / ISSUE; ++q) {
-              if (q < LB) load_b(q);
-              else load_a(q - LB);
-            }
+            for (int q = (s - FIRST) * LB / (ISSUE - FIRST); q < (s + 1 - FIRST) * LB / (ISSUE - FIRST); ++q) load_b(q);
           }
           if (s == STEPS - 2) {
             next_b();
