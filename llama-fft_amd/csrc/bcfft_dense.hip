@@ -116,19 +116,22 @@ __global__ __launch_bounds__(256) void bc_dense_pack_kernel(const char* __restri
 
 // ------------------------------------------------------------------ launches
 // Tile and slices for an m x n product over ksteps tiles of k, with `parts` products per output (2: gated):
-// the least estimated time in microseconds. A CU's time for one tile of k of one workgroup is idle + busy u, u
-// the part of the chip's slots that is taken over the call (the clock and the caches give way under load:
-// 256 x 256 tiles 1.06 us at u = 0.44, 1.30 at 0.78, 1.45 at 1); fixed: a workgroup's start and its outputs.
-// 16-bit values fitted to 4096 x 4096 x 4096, 8192 x 4096 x 4096, 1700 x 4096 x 11008, 1700 x 2 (11008) x 4096 and
-// 2048 x 4096 x 64, fp32 to 2048 x 4096 x 64 and 1024, 4096 x 4096 x 1024 and 5963 x 6240 x 128: all within 5 %
-// (k = 64 aside). cols: operands that lie by columns, 0.06 us each. Slices pay their partial sums' way through
-// memory and the finishing launch (1700 x 4096 x 22016 in two: 262 + 13 us, whole 301).
+// the least estimated time in microseconds. A CU's time for one tile of k of one workgroup is
+//   idle + busy u     u: the part of the chip's slots taken over the call; the clock and the caches give way
+//                     under load (256 x 256 tiles: 1.22 us at u = 0.59, 1.29 at 0.78, 1.46 at 1)
+//   + alone           where every CU runs one workgroup: all wait for the same k from HBM, none fills in
+//   + 0.06 cols       operands that lie by columns
+// and fixed a workgroup's start and its outputs. 16-bit values are fitted with weights out of HBM, as a model's
+// are (four to fourteen sets of operands in turn; 1700 and 2048 x 4096 x 4096 and 11008, 1700 x 11008 x 4096,
+// 1700 x 5120 x 13824, 8192 x 4096 x 4096, 1700 x 2 (11008) x 4096): most within 5 %, single rounds of half a
+// chip within 15 %. fp32: 2048 x 4096 x 64 and 1024, 4096 x 4096 x 1024, 5963 x 6240 x 128. Slices pay their
+// partial sums' way through memory and the finishing launch (1700 x 4096 x 11008 in two 142 + 12 us, whole 162).
 static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int cols) {
   if (cols == 0 && m <= 32) return {0, 1};
   const int64_t cus = device_cu_count();
-  struct Kind { int kind, bm, bn; double idle, busy, fixed, step32, fixed32; };
-  const Kind kinds[3] = {{1, 128, 128, 0.46, 0.0, 2.5, 1.85, 4.5}, {2, 256, 128, 0.35, 0.49, 3.0, 3.72, 9.6},
-                         {3, 256, 256, 0.75, 0.70, 6.0, 7.3, 16.0}};
+  struct Kind { int kind, bm, bn; double idle, busy, alone, fixed, step32, alone32, fixed32; };
+  const Kind kinds[3] = {{1, 128, 128, 0.30, 0.20, 0.12, 2.5, 1.85, 0.28, 4.5}, {2, 256, 128, 0.46, 0.40, 0.10, 3.0, 3.72, 0.0, 9.6},
+                         {3, 256, 256, 0.90, 0.56, 0.06, 6.0, 7.3, 0.0, 16.0}};
   Shape best{1, 1};
   double least = 1e300;
   for (const Kind& q : kinds) {
@@ -138,7 +141,7 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
       const int64_t per_cu = (groups + cus - 1) / cus;                   // the fullest CU's workgroups
       const double used = (double)groups / (double)(per_cu * cus);
       double step = dt == BCFFT_F32 ? q.step32 : q.idle + q.busy * used + 0.06 * cols;
-      if (q.kind == 1 && per_cu == 1) step *= dt == BCFFT_F32 ? 1.15 : 1.3;    // two of these share a CU's gaps
+      if (per_cu == 1) step += dt == BCFFT_F32 ? q.alone32 : q.alone;
       double cost = (double)per_cu * ((double)((ksteps + kz - 1) / kz) * step + (dt == BCFFT_F32 ? q.fixed32 : q.fixed));
       if (kz > 1) cost += 4.0 + (double)(2 * kz) * m * n * parts * 4.0 / 5e6;
       if (cost < least) {
