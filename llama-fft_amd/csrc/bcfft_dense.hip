@@ -126,7 +126,11 @@ __global__ __launch_bounds__(256) void bc_dense_pack_kernel(const char* __restri
 // 1700 x 5120 x 13824, 8192 x 4096 x 4096, 1700 x 2 (11008) x 4096): most within 5 %, single rounds of half a
 // chip within 15 %. fp32: 2048 x 4096 x 64 and 1024, 4096 x 4096 x 1024, 5963 x 6240 x 128. Slices pay their
 // partial sums' way through memory and the finishing launch (1700 x 4096 x 11008 in two 142 + 12 us, whole 162).
-static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int cols) {
+// Up to 32 rows run the few-rows kernel; up to 64 where it takes less than tiles of 128 rows with `pack`, the
+// packing of their operands: all of x passes through every CU that has a workgroup, 16 rows of W at a time
+// (16-bit 48 x 4096 -> 4096: 20.6 us against 16.8, with 4954 features, packed, 30.4 against 36.8; fp32 37.6
+// against 47.0, 56.9 against 80.9).
+static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int cols, double pack = 0.0) {
   if (cols == 0 && m <= 32) return {0, 1};
   const int64_t cus = device_cu_count();
   struct Kind { int kind, bm, bn; double idle, busy, alone, fixed, step32, alone32, fixed32; };
@@ -134,6 +138,11 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
                          {3, 256, 256, 0.90, 0.56, 0.06, 6.0, 7.3, 0.0, 16.0}};
   Shape best{1, 1};
   double least = 1e300;
+  if (cols == 0 && m <= 64) {
+    const int64_t rounds = ((n + 15) / 16 + cus - 1) / cus;
+    least = (double)(rounds * ksteps) * (0.09 + 0.0044 * (double)m + 0.05 * (parts - 1)) + 1.5 - pack;
+    best = {0, 1};
+  }
   for (const Kind& q : kinds) {
     const int64_t tiles = ((m + q.bm - 1) / q.bm) * ((n * parts + q.bn - 1) / q.bn);
     for (int64_t kz = 1; kz <= 16 && (kz == 1 || ksteps / kz >= 4); ++kz) {
@@ -143,7 +152,7 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
       double step = dt == BCFFT_F32 ? q.step32 : q.idle + q.busy * used + 0.06 * cols;
       if (per_cu == 1) step += dt == BCFFT_F32 ? q.alone32 : q.alone;
       double cost = (double)per_cu * ((double)((ksteps + kz - 1) / kz) * step + (dt == BCFFT_F32 ? q.fixed32 : q.fixed));
-      if (kz > 1) cost += 4.0 + (double)(2 * kz) * m * n * parts * 4.0 / 5e6;
+      if (kz > 1) cost += 6.0 + (double)(2 * kz) * m * n * parts * 4.0 / 5e6;
       if (cost < least) {
         least = cost;
         best = {q.kind, (int)kz};
@@ -195,7 +204,9 @@ struct ForwardPlan {
 };
 static ForwardPlan forward_plan(int64_t n, int64_t k, int64_t m, int dt, int parts) {
   ForwardPlan p;
-  p.shape = choose(n, m, ksteps(k, dt), parts, dt, 0);
+  // two launches, and the operands read and written once more
+  const double pack = whole(k, dt) ? 0.0 : 5.0 + (double)(2 * packed_bytes(n + parts * m, k, dt)) / 4.6e6;
+  p.shape = choose(n, m, ksteps(k, dt), parts, dt, 0, pack);
   p.packed = p.shape.kind != 0 && !whole(k, dt);       // the few-rows kernel reads any address
   p.pack_bytes = p.packed ? packed_bytes(n + parts * m, k, dt) : 0;
   p.total = p.pack_bytes + partial_bytes(n, parts * m, p.shape);

@@ -29,13 +29,14 @@ __global__ __launch_bounds__(256) void bc_dense_finish_kernel(DenseArgs a) {
 // Up to 16 MT rows of x (decode): bound by the weights' single read. A workgroup takes 16 rows of W (and 16
 // of the other weight, GLU), its KW waves a part of k each, straight from memory into the fragments; x comes
 // out of L2. The waves' sums meet in LDS.
+// Past 32 rows x's traffic out of L2 outweighs W's, and two tiles of k at a time fill the registers.
 // A wave with few 128-byte tiles of k (8 for 4096 16-bit values) loads four at a time; with more (STREAM) it
 // loads one while it multiplies the last: 1 x 4096 -> 2 x 11008 36.9 us against 34.1 from HBM (5.3 TB/s), 1 x
 // 11008 -> 4096 22.7 against 20.3, but 1 x 4096 -> 4096 6.6 against 7.0 and every two-row-tile form.
 template <int DT, int MT, int KW, bool STREAM, bool GLU>
 __global__ __launch_bounds__(64 * KW) void bc_dense_rows_kernel(DenseArgs a) {
   constexpr int E = DT == BCFFT_F32 ? 4 : 2, EPC = 16 / E, BK = 128 / E, NB = GLU ? 2 : 1;
-  constexpr int UNROLL = 4;
+  constexpr int UNROLL = MT > 2 ? 2 : 4;
   __shared__ f32x4 part[KW][NB * MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l = lane & 15;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
@@ -191,18 +192,18 @@ static void launch_rows(const DenseArgs& a, hipStream_t s) {
   using std::bool_constant;
   const integral_constant<int, 1> one;
   const integral_constant<int, 2> two;
-  const integral_constant<int, 4> kw4;
-  const integral_constant<int, 8> kw8;
+  const integral_constant<int, 3> three;
+  const integral_constant<int, 4> four;
   // 8 waves per 16 rows of W while that leaves no more than two workgroups per CU, 4 beyond
-  if (groups <= 512) {
-    if (a.m > 16) go(two, kw8, bool_constant<false>());
-    else if (tiles >= 12 * 8) go(one, kw8, bool_constant<true>());
-    else go(one, kw8, bool_constant<false>());
-  } else {
-    if (a.m > 16) go(two, kw4, bool_constant<false>());
-    else if (tiles >= 12 * 4) go(one, kw4, bool_constant<true>());
-    else go(one, kw4, bool_constant<false>());
-  }
+  auto with = [&](auto kw) {
+    if (a.m > 48) go(four, kw, bool_constant<false>());
+    else if (a.m > 32) go(three, kw, bool_constant<false>());
+    else if (a.m > 16) go(two, kw, bool_constant<false>());
+    else if (tiles >= 12 * kw.value) go(one, kw, bool_constant<true>());
+    else go(one, kw, bool_constant<false>());
+  };
+  if (groups <= 512) with(integral_constant<int, 8>());
+  else with(integral_constant<int, 4>());
 }
 
 template <int DT>

@@ -486,3 +486,21 @@ def test_two_streams_at_once(dev):
     for i in range(2):
         for out in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("n,k,m", [(33, 129, 40), (40, 2049, 130), (48, 96, 17), (49, 1003, 64), (64, 777, 33),
+                                   (64, 4096, 24), (61, 130, 9000), (65, 777, 33)])
+def test_33_to_64_rows(dev, dt, n, k, m):
+    """Both sides of the rule between the few-rows kernel and tiles, with rows that need packing and without."""
+    from bcfft import dense
+    x, w, wu = (rand(dev, *s, dt=DT[dt], seed=111 + i, scale=c) for i, (s, c) in
+                enumerate((((n, k), 1.0), ((m, k), k ** -0.5), ((m, k), k ** -0.5))))
+    b, r = rand(dev, m, dt=DT[dt], seed=115), rand(dev, n, m, dt=DT[dt], seed=116)
+    want, slack, *_ = linear64(x, w, b, r, "gelu")
+    within(dense.linear(x, w, b, activation="gelu", residual=r), want, slack)
+    x64, w64, u64 = x.double(), w.double(), wu.double()
+    g, u = x64 @ w64.t(), x64 @ u64.t()
+    v, _ = act64(g, "silu")
+    gs, us = sum_slack(x64, w64.t()), sum_slack(x64, u64.t())
+    within(dense.glu(x, w, wu), v * u, (1.2 * gs + 16 * U * v.abs()) * u.abs() + v.abs() * us + U * (v * u).abs())
