@@ -224,7 +224,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void bc_dense_tile_kernel(DenseArg
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr int STEPS = 2 * FM, HALF = FN + (FM > FN ? 2 : 0);
-  static_assert(FN <= FM && HALF < STEPS - 2, "B's second half is read before its buffer is loaded anew");
+  constexpr int PER_STEP = FN > FM ? FN / FM : 1;      // B's second fragments, read in the first FM steps
+  static_assert(FN <= FM * PER_STEP && (!REUSE || (PER_STEP == 1 && HALF < STEPS - 2)), "and before its buffer is loaded anew");
   uint4 va[4], vb[2][FN];
   auto read_a = [&](const char* tile, int s) { return fa.read(tile, wm * TM + s % FM * 16, s / FM); };
   auto read_b = [&](const char* tile, int j, int kk) {
@@ -293,13 +294,15 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void bc_dense_tile_kernel(DenseArg
         const char* tb = lds_b + rb;
         ra = ra + ABYTES == RA * ABYTES ? 0 : ra + ABYTES;
         rb = rb + BBYTES == RB * BBYTES ? 0 : rb + BBYTES;
-        constexpr int ISSUE = STEPS - 2, FIRST = REUSE ? HALF : ISSUE * LA / (LA + LB);
+        constexpr int ISSUE = STEPS - 2, SHARE = ISSUE * LA / (LA + LB), FIRST = REUSE ? HALF : SHARE > 0 ? SHARE : 1;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
           const int kk = s / FM, i = s % FM;
           if (REUSE && s == HALF) tile_reuse();        // every wave holds B's fragments
           if (s + 2 < STEPS) va[(s + 2) % 4] = read_a(ta, s + 2);
-          if (s < FN) vb[1][s] = read_b(tb, s, 1);
+#pragma unroll
+          for (int j = s * PER_STEP; j < (s + 1) * PER_STEP; ++j)
+            if (j < FN) vb[1][j] = read_b(tb, j, 1);
           if (s < FIRST) {
 #pragma unroll
             for (int q = s * LA / FIRST; q < (s + 1) * LA / FIRST; ++q) load_a(q);
