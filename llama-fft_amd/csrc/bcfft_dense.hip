@@ -225,7 +225,7 @@ static BackwardPlan backward_plan(int64_t n, int64_t k, int64_t m, int dt, int p
   BackwardPlan p;
   const bool split = parts == 2 && !whole(m, dt);      // dg and du are not adjacent columns
   p.dx = choose(n, k, parts * ksteps(m, dt), 1, dt, 1);
-  p.dw = choose(split ? m : parts * m, k, ksteps(n, dt), 1, dt, 2);
+  p.dw = n <= 32 ? Shape{0, 1} : choose(split ? m : parts * m, k, ksteps(n, dt), 1, dt, 2);
   p.dz_bytes = parts == 2 || act != BCFFT_ACT_NONE || !whole(m, dt) ? parts * packed_bytes(n, m, dt) : 0;
   // 64 rows per workgroup of dz where that makes four workgroups per CU, else 16 (2048 x 4096: 25 -> 18 us, 1362 x 448: 18 -> 6 us)
   p.rows = (n + 63) / 64 * ((m + 255) / 256) >= 4 * device_cu_count() ? 64 : 16;

@@ -504,3 +504,15 @@ def test_33_to_64_rows(dev, dt, n, k, m):
     v, _ = act64(g, "silu")
     gs, us = sum_slack(x64, w64.t()), sum_slack(x64, u64.t())
     within(dense.glu(x, w, wu), v * u, (1.2 * gs + 16 * U * v.abs()) * u.abs() + v.abs() * us + U * (v * u).abs())
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("n,k,m", [(1, 260, 300), (5, 4099, 16500), (31, 515, 70), (32, 4096, 513), (33, 130, 70)])
+def test_few_tokens_weight_gradient(dev, dt, n, k, m):
+    """Up to 32 tokens: whole and ragged blocks of 256 columns, 64 and 256 rows per workgroup."""
+    from bcfft import dense
+    x, w = rand(dev, n, k, dt=DT[dt], seed=121), rand(dev, m, k, dt=DT[dt], seed=122, scale=k ** -0.5).requires_grad_()
+    dy = rand(dev, n, m, dt=DT[dt], seed=123)
+    dense.linear(x, w).backward(dy)
+    d64, x64 = dy.double(), x.double()
+    within(w.grad, d64.t() @ x64, sum_slack(d64.t(), x64))
