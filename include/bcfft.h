@@ -302,7 +302,7 @@ int bcfft_distill_topk_backward(const void* logits, int dtype, int64_t n_rows, i
  * in_features) contiguous; bias (out_features) or NULL; residual (n_tokens, out_features) with r_stride, or
  * NULL; y / h (n_tokens, out_features) contiguous. Everything of one dtype. x, the weights and dy start on 16
  * bytes, and so do the rows of x and dy where their features fill whole 16-byte pieces; other features are
- * copied to padded rows in the workspace first (the forwards of up to 32 rows read them as they are). The
+ * copied to padded rows in the workspace first (the forwards of few rows, up to 32 and some up to 64, read them as they are). The
  * rest is element-aligned. Products accumulate in fp32, bias, activation and residual are
  * applied there, one rounding to dtype. Features and strides up to 2^20 (the glu backward: 2 out_features), up to 2^23
  * tokens; n_tokens == 0 is a no-op.

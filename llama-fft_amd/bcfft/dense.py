@@ -153,9 +153,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
 
     x (..., in_features), weight (out_features, in_features), bias (out_features), residual (...,
     out_features), all float32, float16 or bfloat16 alike, any sizes up to 2^20 features. activation: None,
-    "relu", "silu" or "gelu" (exact). fp32 accumulation, one rounding. Up to 32 rows run the weight-streaming
-    kernel. The gradient of an activation's input is rounded once to the dtype before the two products that
-    read it; bias gradients sum the unrounded values."""
+    "relu", "silu" or "gelu" (exact). fp32 accumulation, one rounding. Up to 32 rows (64 where
+    it pays) run the weight-streaming kernel. The gradient of an activation's input is rounded once to the
+    dtype before the two products that read it; bias gradients sum the unrounded values."""
     if _lib.native_op():                         # the same call as one C++ op (csrc/bcfft_torch_ops.cpp)
         return _lib.NATIVE_OPS["dense_linear"](x, weight, bias, residual, _activation("bcfft.dense.linear", activation))
     lead = x.shape[:-1]
