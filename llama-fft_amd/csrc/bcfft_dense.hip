@@ -414,9 +414,10 @@ int bcfft_dense_linear_backward(const void* x, int dtype, int64_t n_tokens, int6
   const int64_t ldg = dz ? mp : dy_stride;
   const bool packed = p.pack_bytes > 0;
   const void* wp = packed && dx ? pack(dtype, w, k, m, k, ws, s) : w;
-  const void* xp = packed && dw ? pack(dtype, x, x_stride, n, k, ws, s) : x;
+  const bool xpacked = packed && p.dw.kind != 0;       // few tokens' weight gradient reads any address
+  const void* xp = xpacked && dw ? pack(dtype, x, x_stride, n, k, ws, s) : x;
   if (dx) launch_dx(dtype, g, ldg, 0, wp, nullptr, n, k, packed ? kp : k, m, p.dx, dx, (float*)ws, s);
-  if (dw) launch_dw(dtype, g, ldg, dz ? mp : m, xp, packed ? kp : x_stride, packed ? kp : k, n, k, m, p.dw, dw, (float*)ws, s);
+  if (dw) launch_dw(dtype, g, ldg, dz ? mp : m, xp, xpacked ? kp : x_stride, xpacked ? kp : k, n, k, m, p.dw, dw, (float*)ws, s);
   return record_launch_status();
 }
 
@@ -448,9 +449,10 @@ int bcfft_dense_glu_backward(const void* x, int dtype, int64_t n_tokens, int64_t
   const bool packed = p.pack_bytes > 0;
   const void* wgp = packed && dx ? pack(dtype, w_gate, k, m, k, ws, s) : w_gate;
   const void* wup = packed && dx ? pack(dtype, w_up, k, m, k, ws, s) : w_up;
-  const void* xp = packed && dw ? pack(dtype, x, x_stride, n, k, ws, s) : x;
-  const int64_t ldx = packed ? kp : x_stride, kr = packed ? kp : k;
-  if (dx) launch_dx(dtype, dz, 2 * mp, mp, wgp, wup, n, k, kr, m, p.dx, dx, (float*)ws, s);
+  const bool xpacked = packed && p.dw.kind != 0;       // few tokens' weight gradient reads any address
+  const void* xp = xpacked && dw ? pack(dtype, x, x_stride, n, k, ws, s) : x;
+  const int64_t ldx = xpacked ? kp : x_stride, kr = xpacked ? kp : k;
+  if (dx) launch_dx(dtype, dz, 2 * mp, mp, wgp, wup, n, k, packed ? kp : k, m, p.dx, dx, (float*)ws, s);
   if (dw && mp == m) {
     launch_dw(dtype, dz, 2 * mp, 2 * mp, xp, ldx, kr, n, k, 2 * m, p.dw, dw, (float*)ws, s);
   } else if (dw) {
