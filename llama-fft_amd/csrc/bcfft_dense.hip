@@ -128,10 +128,10 @@ __global__ __launch_bounds__(256) void bc_dense_pack_kernel(const char* __restri
 // partial sums' way through memory and the finishing launch (1700 x 4096 x 11008 in two 142 + 12 us, whole 162).
 // Few rows leave most of a 128-row tile's products empty, which fp32 pays for (4096 -> 4096, by columns: 20 rows
 // 38.6 us, 24.0 in 64-row tiles, 19.6 in 32-row tiles; bf16 13.1, 12.1, 11.5).
-// Up to 32 rows run the few-rows kernel; up to 64 where it takes less than tiles of 128 rows with `pack`, the
+// Up to 32 rows run the few-rows kernel; more, 64 at a time, where that takes less than tiles with `pack`, the
 // packing of their operands: all of x passes through every CU that has a workgroup, 16 rows of W at a time
-// (16-bit 48 x 4096 -> 4096: 20.6 us against 16.8, with 4954 features, packed, 30.4 against 36.8; fp32, packed,
-// 56.9 against 80.9).
+// (16-bit 48 x 4096 -> 4096: 20.6 us against 16.8, with 4954 features, packed, 30.4 against 36.8; 512 x 512 -> 512
+// 5.0 against 8.6; fp32 48 x 4954 -> 4096 56.9 against 80.9, 512 x 512 -> 512 7.5 against 18.1).
 static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int cols, double pack = 0.0) {
   if (cols == 0 && m <= 32) return {0, 1};
   const int64_t cus = device_cu_count();
@@ -139,15 +139,17 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
   const Kind kinds[5] = {{1, 128, 128, 0.30, 0.20, 0.12, 2.5, 1.85, 0.28, 4.5}, {2, 256, 128, 0.46, 0.40, 0.10, 3.0, 3.72, 0.0, 9.6},
                          {3, 256, 256, 0.90, 0.56, 0.06, 6.0, 7.3, 0.0, 16.0}, {4, 64, 128, 0.28, 0.18, 0.12, 2.5, 0.95, 0.25, 3.0},
                          {5, 32, 128, 0.26, 0.16, 0.12, 2.5, 0.50, 0.45, 3.0}};
+  constexpr double START = 2.0;                        // of a tile launch beyond the few-rows kernel's
   Shape best{1, 1};
   double least = 1e300;
-  if (cols == 0 && m <= 64) {
-    const int64_t rounds = ((n + 15) / 16 + cus - 1) / cus;
-    least = (double)(rounds * ksteps) * (0.09 + 0.0044 * (double)m + 0.05 * (parts - 1)) + 1.5 - pack;
+  if (cols == 0) {
+    const int64_t rounds = ((n + 15) / 16 * ((m + 63) / 64) + cus - 1) / cus;
+    const double rows = m < 64 ? (double)m : 64.0;
+    least = (double)(rounds * ksteps) * (0.09 + 0.0044 * rows + 0.05 * (parts - 1)) + 1.5 - pack - START;
     best = {0, 1};
   }
   for (const Kind& q : kinds) {
-    if ((q.kind == 4 && (cols == 2 || m > 64)) || (q.kind == 5 && (cols != 1 || m > 32))) continue;
+    if ((q.kind == 4 && cols == 2) || (q.kind == 5 && (cols != 1 || m > 32))) continue;
     const int64_t tiles = ((m + q.bm - 1) / q.bm) * ((n * parts + q.bn - 1) / q.bn);
     for (int64_t kz = 1; kz <= 16 && (kz == 1 || ksteps / kz >= 4); ++kz) {
       const int64_t groups = tiles * kz;

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void bc_dense_finish_kernel(DenseArgs a) {
 }
 
 // ------------------------------------------------------------------ few rows
-// Up to 16 MT rows of x (decode): bound by the weights' single read. A workgroup takes 16 rows of W (and 16
+// 16 MT rows of x (decode; more rows: one block of them per grid row): bound by the weights' single read. A workgroup takes 16 rows of W (and 16
 // of the other weight, GLU), its KW waves a part of k each, straight from memory into the fragments; x comes
 // out of L2. The waves' sums meet in LDS.
 // Past 32 rows x's traffic out of L2 outweighs W's, and two tiles of k at a time fill the registers.
@@ -39,14 +39,14 @@ __global__ __launch_bounds__(64 * KW) void bc_dense_rows_kernel(DenseArgs a) {
   constexpr int UNROLL = MT > 2 ? 2 : 4;
   __shared__ f32x4 part[KW][NB * MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l = lane & 15;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MT;
   const int64_t wrow = n0 + l < a.n ? n0 + l : a.n - 1;       // repeated rows are not stored
   const char* pw[NB];
 #pragma unroll
   for (int s = 0; s < NB; ++s) pw[s] = (const char*)a.b[s] + wrow * a.ldb * E;
   const char* px[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) px[i] = (const char*)a.a[0] + (16 * i + l < a.m ? 16 * i + l : a.m - 1) * a.lda * E;
+  for (int i = 0; i < MT; ++i) px[i] = (const char*)a.a[0] + (m0 + 16 * i + l < a.m ? m0 + 16 * i + l : a.m - 1) * a.lda * E;
   const int64_t tiles = (a.k + BK - 1) / BK;
   const int64_t t0 = tiles * wave / KW, t1 = tiles * (wave + 1) / KW;
 
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * KW) void bc_dense_rows_kernel(DenseArgs a) {
     for (int i = 0; i < MT; ++i) part[wave][s * MT + i][lane] = acc[s][i];
   __syncthreads();
   for (int i = wave; i < MT; i += KW) {
-    const int64_t m = 16 * i + l, n = n0 + 4 * g;
+    const int64_t m = m0 + 16 * i + l, n = n0 + 4 * g;
     if (m >= a.m || n >= a.n) continue;
     float v[NB][4];
 #pragma unroll
@@ -262,7 +262,8 @@ static void launch_rows(const DenseArgs& a, hipStream_t s) {
   const unsigned groups = (unsigned)((a.n + 15) / 16);
   const int64_t tiles = (a.k * (DT == BCFFT_F32 ? 4 : 2) + 127) / 128;
   auto go = [&](auto mt, auto kw, auto stream) {
-    hipLaunchKernelGGL((bc_dense_rows_kernel<DT, mt.value, kw.value, stream.value, GLU>), dim3(groups), dim3(64 * kw.value), 0, s, a);
+    hipLaunchKernelGGL((bc_dense_rows_kernel<DT, mt.value, kw.value, stream.value, GLU>), dim3(groups, (unsigned)((a.m + 16 * mt.value - 1) / (16 * mt.value))),
+                       dim3(64 * kw.value), 0, s, a);
   };
   using std::integral_constant;
   using std::bool_constant;

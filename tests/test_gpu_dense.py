@@ -516,3 +516,21 @@ def test_few_tokens_weight_gradient(dev, dt, n, k, m):
     dense.linear(x, w).backward(dy)
     d64, x64 = dy.double(), x.double()
     within(w.grad, d64.t() @ x64, sum_slack(d64.t(), x64))
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("n,k,m", [(65, 64, 1040), (129, 520, 50), (300, 2008, 1100), (700, 136, 2000), (193, 4104, 4100),
+                                   (1025, 72, 100)])
+def test_more_than_64_rows(dev, dt, n, k, m):
+    """Blocks of 64 rows of the few-rows kernel, and tiles, with ends inside them."""
+    from bcfft import dense
+    x, w, wu = (rand(dev, *s, dt=DT[dt], seed=131 + i, scale=c) for i, (s, c) in
+                enumerate((((n, k), 1.0), ((m, k), k ** -0.5), ((m, k), k ** -0.5))))
+    b, r = rand(dev, m, dt=DT[dt], seed=135), rand(dev, n, m, dt=DT[dt], seed=136)
+    want, slack, *_ = linear64(x, w, b, r, "silu")
+    within(dense.linear(x, w, b, activation="silu", residual=r), want, slack)
+    x64, w64, u64 = x.double(), w.double(), wu.double()
+    g, u = x64 @ w64.t(), x64 @ u64.t()
+    v, _ = act64(g, "gelu")
+    gs, us = sum_slack(x64, w64.t()), sum_slack(x64, u64.t())
+    within(dense.glu(x, w, wu, activation="gelu"), v * u, (1.2 * gs + 16 * U * v.abs()) * u.abs() + v.abs() * us + U * (v * u).abs())
