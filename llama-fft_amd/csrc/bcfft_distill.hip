@@ -212,11 +212,13 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 1. The largest logit of each thread or, for k <= 128, of each of 256 groups of threads; the k-th largest of
-//    these bounds the k-th largest element from below (k groups hold at least one that large each), and
-//    hardly more than k elements reach it (74 for k = 64 of 256, evenly spread). Its upper 16 bits are enough:
-//    one wave finds it bit by bit, by ballots over G / 64 maxima per lane (16 of them: 8000 of the kernel's
-//    29000 clocks at 20 x 32000, which is why there are no more than 4 where k allows it). 1.5 operations a logit
+// 1. The largest logit of each thread (of 1024 threads: of each half of its pieces) or, for k <= 128, of each of
+//    256 groups of threads: at least 2 k maxima. The k-th largest of them bounds the k-th largest element from
+//    below (k groups hold at least one that large each), and hardly more than k elements reach it (74 for k = 64
+//    of 256, evenly spread; but 900 for k = 249 of 256: 1609 x 2960 fp32 195 us, 51 with 512). Its upper 16 bits
+//    are enough: one wave finds it bit by bit, by ballots over G / 64 maxima per lane (16 of them took 8000 of
+//    the kernel's 29000 clocks at 20 x 32000, so there are no more than 4 where k allows it).
+//                                                                                  1.5 operations a logit
 // 2. The elements at or above the bound go to LDS, the others' exponentials relative to it are summed.    9
 // 3. Each candidate counts the candidates above it: its rank is its place in the output. Ranks depend on
 //    keys alone, so the order of arrival does not matter.
@@ -229,13 +231,14 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
                                                             void* __restrict__ values, int32_t* __restrict__ indices,
                                                             float* __restrict__ rest) {
   constexpr int E = DT == BCFFT_F32 ? 4 : 2;
-  constexpr int TOPK_CAND = NT == 256 ? 1024 : 2048;     // candidates ranked in LDS (k <= NT)
+  constexpr int TOPK_CAND = NT == 256 ? 1024 : 2048;     // candidates ranked in LDS
+  constexpr bool TWO = NT == 1024;
   constexpr int VEC = RowType<DT>::VEC, CHUNK = HOLD > 0 ? 64 / VEC : 1;    // pieces per 64-bit mask
   __shared__ int at_s[TOPK_CAND];        // the candidates: indices, as they come
   __shared__ uint64_t cand[TOPK_CAND];   // their keys
   __shared__ uint32_t raw[TOPK_CAND];    // their logits as they stand in the row
   __shared__ float left[TOPK_CAND];
-  __shared__ uint32_t gmax[NT];
+  __shared__ uint32_t gmax[TWO ? 2 * NT : NT];
   __shared__ uint32_t redu[NT / 64];
   __shared__ float redf[NT / 64];
   __shared__ double redd[NT / 64];
@@ -247,17 +250,21 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
   Row<DT, NT, HOLD> r;
   r.open(row, vocab);
 
-  float best = -INFINITY;                // NaN passes it by: it still is a candidate below
-  bool any = false;
+  float best = -INFINITY, second = -INFINITY;        // NaN passes them by: it still is a candidate below
+  int seen = 0;                          // pieces; with TWO the odd ones' maximum is kept apart
   r.each([&](int, auto& v) {
-    any = true;
+    float mx = v[0];
+    if constexpr (count_of<decltype(v)> > 1) mx = fmaxf(mx, v[1]);
 #pragma unroll
-    for (int j = 0; j + 1 < count_of<decltype(v)>; j += 2) best = fmaxf(fmaxf(best, v[j]), v[j + 1]);
-    if constexpr (count_of<decltype(v)> == 1) best = fmaxf(best, v[0]);
+    for (int j = 2; j + 1 < count_of<decltype(v)>; j += 2) mx = fmaxf(fmaxf(mx, v[j]), v[j + 1]);
+    if (TWO && (seen & 1)) second = fmaxf(second, mx);
+    else best = fmaxf(best, mx);
+    ++seen;
   });
   // 0 is below every key of a number
-  uint32_t key = any ? order_key(best) : 0;
   const bool grouped = NT > 256 && k <= 128;
+  uint32_t key = seen ? order_key(grouped ? fmaxf(best, second) : best) : 0;
+  if (TWO && !grouped) gmax[NT + tid] = seen > 1 ? order_key(second) : 0;
   if (grouped) {
     key = lanes_reduce<NT / 256>(key, MaxOp());
     if (tid % (NT / 256) == 0) gmax[tid / (NT / 256)] = key;
@@ -282,7 +289,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
       if (tid == 0) bound_s = (int)b;
     };
     if (grouped) search(std::integral_constant<int, 4>());
-    else search(std::integral_constant<int, NT / 64>());
+    else search(std::integral_constant<int, (TWO ? 2 : 1) * NT / 64>());
   }
   __syncthreads();
   // an element reaches the bound unless it is less: NaN does, and without a bound all do
@@ -801,12 +808,12 @@ static ExpScale exp_scale(double temperature) {
 // Threads and pieces per thread by the row's number of 16-byte pieces: the fewest threads that hold it
 // with 8 pieces each (more rows per CU), then 16 pieces, then a row that is read again.
 template <int DT, class F>
-static void by_row(int64_t vocab, int64_t min_threads, F&& go) {
+static void by_row(int64_t vocab, F&& go) {
   const int64_t pieces = (vocab + RowType<DT>::VEC - 1) / RowType<DT>::VEC;
   using std::integral_constant;
-  if (pieces <= 512 && min_threads <= 256) go(integral_constant<int, 256>(), integral_constant<int, 2>());
-  else if (pieces <= 2048 && min_threads <= 256) go(integral_constant<int, 256>(), integral_constant<int, 8>());
-  else if (pieces <= 4096 && min_threads <= 512) go(integral_constant<int, 512>(), integral_constant<int, 8>());
+  if (pieces <= 512) go(integral_constant<int, 256>(), integral_constant<int, 2>());
+  else if (pieces <= 2048) go(integral_constant<int, 256>(), integral_constant<int, 8>());
+  else if (pieces <= 4096) go(integral_constant<int, 512>(), integral_constant<int, 8>());
   else if (pieces <= 8192) go(integral_constant<int, 1024>(), integral_constant<int, 8>());
   else if (pieces <= 16384) go(integral_constant<int, 1024>(), integral_constant<int, 16>());
   else go(integral_constant<int, 1024>(), integral_constant<int, 0>());
@@ -819,11 +826,33 @@ static void by_rows(int64_t n, F&& go) {
   for (int64_t first = 0; first < n; first += LAUNCH_ROWS) go(first, n - first < LAUNCH_ROWS ? n - first : LAUNCH_ROWS);
 }
 
+// The same for the top k, with at least 2 k threads (k <= 512)
+template <int DT, class F>
+static void by_row_topk(int64_t vocab, int64_t k, F&& go) {
+  const int64_t pieces = (vocab + RowType<DT>::VEC - 1) / RowType<DT>::VEC;
+  using std::integral_constant;
+  if (2 * k <= 256 && pieces <= 2048) {
+    if (pieces <= 512) go(integral_constant<int, 256>(), integral_constant<int, 2>());
+    else go(integral_constant<int, 256>(), integral_constant<int, 8>());
+  } else if (2 * k <= 512 && pieces <= 4096) {
+    if (pieces <= 1024) go(integral_constant<int, 512>(), integral_constant<int, 2>());
+    else go(integral_constant<int, 512>(), integral_constant<int, 8>());
+  } else if (pieces <= 2048) {
+    go(integral_constant<int, 1024>(), integral_constant<int, 2>());
+  } else if (pieces <= 8192) {
+    go(integral_constant<int, 1024>(), integral_constant<int, 8>());
+  } else if (pieces <= 16384) {
+    go(integral_constant<int, 1024>(), integral_constant<int, 16>());
+  } else {
+    go(integral_constant<int, 1024>(), integral_constant<int, 0>());
+  }
+}
+
 template <int DT>
 static void launch_topk_dt(const void* logits, int64_t n, int64_t vocab, int64_t row_stride, int k, double temperature,
                            void* values, int32_t* indices, float* rest, hipStream_t s) {
   constexpr int64_t E = DT == BCFFT_F32 ? 4 : 2;
-  by_row<DT>(vocab, k, [&](auto nt, auto hold) {
+  by_row_topk<DT>(vocab, k, [&](auto nt, auto hold) {
     by_rows(n, [&](int64_t at, int64_t rows) {
       hipLaunchKernelGGL((bc_topk_logits_kernel<DT, nt.value, hold.value>), dim3((unsigned)rows), dim3(nt.value), 0, s,
                          (const char*)logits + at * row_stride * E, vocab, row_stride, k, exp_scale(temperature),
@@ -856,7 +885,7 @@ static void launch_distill_rows(const DistillArgs& a, int64_t n, hipStream_t s) 
     hipLaunchKernelGGL((bc_distill_backward_kernel<DT, 512>), dim3((unsigned)n), dim3(512), lds, s, a);
     return;
   }
-  by_row<DT>(a.vocab, 1, [&](auto nt, auto hold) {
+  by_row<DT>(a.vocab, [&](auto nt, auto hold) {
     if (a.grad) hipLaunchKernelGGL((bc_distill_kernel<DT, nt.value, hold.value, true>), dim3((unsigned)n), dim3(nt.value), lds, s, a);
     else hipLaunchKernelGGL((bc_distill_kernel<DT, nt.value, hold.value, false>), dim3((unsigned)n), dim3(nt.value), lds, s, a);
   });
