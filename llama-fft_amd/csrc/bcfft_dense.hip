@@ -9,6 +9,7 @@
 // of tiles and the C entry points.
 #include "bcfft_dense.h"
 
+#include <cmath>
 #include <type_traits>
 
 namespace bcfft {
@@ -120,12 +121,14 @@ __global__ __launch_bounds__(256) void bc_dense_pack_kernel(const char* __restri
 //   idle + busy u     u: the part of the chip's slots taken over the call; the clock and the caches give way
 //                     under load (256 x 256 tiles: 1.22 us at u = 0.59, 1.29 at 0.78, 1.46 at 1)
 //   + alone           where every CU runs one workgroup: all wait for the same k from HBM, none fills in
-//   + 0.06 cols       operands that lie by columns
+//   + 0.06 cols       operands that lie by columns (by the tile's side)
 // and fixed a workgroup's start and its outputs. 16-bit values are fitted with weights out of HBM, as a model's
 // are (four to fourteen sets of operands in turn; 1700 and 2048 x 4096 x 4096 and 11008, 1700 x 11008 x 4096,
 // 1700 x 5120 x 13824, 8192 x 4096 x 4096, 1700 x 2 (11008) x 4096): most within 5 %, single rounds of half a
 // chip within 15 %. fp32: 2048 x 4096 x 64 and 1024, 4096 x 4096 x 1024, 5963 x 6240 x 128. Slices pay their
 // partial sums' way through memory and the finishing launch (1700 x 4096 x 11008 in two 142 + 12 us, whole 162).
+// Small tiles spread small products: 128 x 1024 -> 4096 takes 12.0 us in 128 x 128 tiles, 9.3 in 64 x 128, 7.4 in 64
+// x 64 (fp32 65.7, 36.8, 21.3); 1024 x 4096 -> 4096 43.3, 50.5, 65.3.
 // Few rows leave most of a 128-row tile's products empty, which fp32 pays for (4096 -> 4096, by columns: 20 rows
 // 38.6 us, 24.0 in 64-row tiles, 19.6 in 32-row tiles; bf16 13.1, 12.1, 11.5).
 // Up to 32 rows run the few-rows kernel; more, 64 at a time, where that takes less than tiles with `pack`, the
@@ -136,9 +139,9 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
   if (cols == 0 && m <= 32) return {0, 1};
   const int64_t cus = device_cu_count();
   struct Kind { int kind, bm, bn; double idle, busy, alone, fixed, step32, alone32, fixed32; };
-  const Kind kinds[5] = {{1, 128, 128, 0.30, 0.20, 0.12, 2.5, 1.85, 0.28, 4.5}, {2, 256, 128, 0.46, 0.40, 0.10, 3.0, 3.72, 0.0, 9.6},
-                         {3, 256, 256, 0.90, 0.56, 0.06, 6.0, 7.3, 0.0, 16.0}, {4, 64, 128, 0.28, 0.18, 0.12, 2.5, 0.95, 0.25, 3.0},
-                         {5, 32, 128, 0.26, 0.16, 0.12, 2.5, 0.50, 0.45, 3.0}};
+  const Kind kinds[6] = {{1, 128, 128, 0.30, 0.20, 0.12, 3.0, 1.85, 0.15, 4.7}, {2, 256, 128, 0.46, 0.40, 0.10, 3.0, 3.72, 0.0, 9.6},
+                         {3, 256, 256, 0.90, 0.56, 0.06, 6.0, 7.3, 0.0, 16.0}, {4, 64, 128, 0.25, 0.09, 0.12, 2.0, 0.95, 0.12, 3.2},
+                         {5, 32, 128, 0.26, 0.16, 0.12, 2.5, 0.50, 0.45, 3.0}, {6, 64, 64, 0.16, 0.08, 0.19, 1.3, 0.47, 0.08, 2.5}};
   constexpr double START = 2.0;                        // of a tile launch beyond the few-rows kernel's
   Shape best{1, 1};
   double least = 1e300;
@@ -149,13 +152,13 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
     best = {0, 1};
   }
   for (const Kind& q : kinds) {
-    if ((q.kind == 4 && cols == 2) || (q.kind == 5 && (cols != 1 || m > 32))) continue;
+    if ((q.kind == 4 && cols == 2) || (q.kind == 5 && (cols != 1 || m > 32)) || (q.kind == 6 && (cols == 2 || parts == 2))) continue;
     const int64_t tiles = ((m + q.bm - 1) / q.bm) * ((n * parts + q.bn - 1) / q.bn);
     for (int64_t kz = 1; kz <= 16 && (kz == 1 || ksteps / kz >= 4); ++kz) {
       const int64_t groups = tiles * kz;
       const int64_t per_cu = (groups + cus - 1) / cus;                   // the fullest CU's workgroups
       const double used = (double)groups / (double)(per_cu * cus);
-      double step = dt == BCFFT_F32 ? q.step32 : q.idle + q.busy * used + 0.06 * cols;
+      double step = dt == BCFFT_F32 ? q.step32 : q.idle + q.busy * used + 0.06 * cols * sqrt(q.bm * q.bn / 65536.0);
       if (per_cu == 1) step += dt == BCFFT_F32 ? q.alone32 : q.alone;
       double cost = (double)per_cu * ((double)((ksteps + kz - 1) / kz) * step + (dt == BCFFT_F32 ? q.fixed32 : q.fixed));
       if (kz > 1) cost += 6.0 + (double)(2 * kz) * m * n * parts * 4.0 / 5e6;

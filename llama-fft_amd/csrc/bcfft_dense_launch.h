@@ -247,8 +247,12 @@ static void launch_tiles(const DenseArgs& a, int kind, hipStream_t s) {
   else if (kind == 2) launch_tile<DT, CA, CB, 256, 128, 4, 2, 3, 3, GLU>(a, s);
   else if (kind == 3) launch_tile<DT, CA, CB, 256, 256, 2, 4, 3, 2, GLU>(a, s);
   else if constexpr (!CA) {
-    if (kind == 4) launch_tile<DT, CA, CB, 64, 128, 2, 2, 3, 3, GLU>(a, s);
-    else if constexpr (CB) launch_tile<DT, CA, CB, 32, 128, 1, 4, 3, 3, GLU>(a, s);
+    if (kind == 4) {
+      launch_tile<DT, CA, CB, 64, 128, 2, 2, 3, 3, GLU>(a, s);
+    } else if constexpr (!GLU) {
+      if (kind == 6) launch_tile<DT, CA, CB, 64, 64, 2, 2, 3, 3, GLU>(a, s);
+      else if constexpr (CB) launch_tile<DT, CA, CB, 32, 128, 1, 4, 3, 3, GLU>(a, s);
+    }
   }
   if (a.kz > 1) {
     const int64_t quads = (a.n + 3) / 4 * a.m;
