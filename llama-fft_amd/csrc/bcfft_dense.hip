@@ -145,7 +145,7 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
   constexpr double START = 2.0;                        // of a tile launch beyond the few-rows kernel's
   Shape best{1, 1};
   double least = 1e300;
-  if (cols == 0) {
+  if (cols == 0 && (m + 63) / 64 <= 65535) {           // blocks of rows are the grid's second dimension
     const int64_t rounds = ((n + 15) / 16 * ((m + 63) / 64) + cus - 1) / cus;
     const double rows = m < 64 ? (double)m : 64.0;
     least = (double)(rounds * ksteps) * (0.09 + 0.0044 * rows + 0.05 * (parts - 1)) + 1.5 - pack - START;

@@ -534,3 +534,12 @@ def test_more_than_64_rows(dev, dt, n, k, m):
     v, _ = act64(g, "gelu")
     gs, us = sum_slack(x64, w64.t()), sum_slack(x64, u64.t())
     within(dense.glu(x, w, wu, activation="gelu"), v * u, (1.2 * gs + 16 * U * v.abs()) * u.abs() + v.abs() * us + U * (v * u).abs())
+
+
+@pytest.mark.parametrize("n", [64 * 65535, 64 * 65535 + 1, 1 << 23])
+def test_millions_of_rows(dev, n):
+    """Blocks of 64 rows up to what one grid dimension holds, and past it."""
+    from bcfft import dense
+    x, w = rand(dev, n, 7, dt=torch.float16, seed=141), rand(dev, 5, 7, dt=torch.float16, seed=142)
+    want = x.double() @ w.double().t()
+    within(dense.linear(x, w), want, sum_slack(x.double(), w.double().t()))
