@@ -458,12 +458,26 @@ def fuse_mlp_gate_up(model) -> int:
     return n
 
 
+def _plain_silu(act) -> bool:
+    """nn.SiLU or transformers' SiLUActivation, computed as these classes do."""
+    if isinstance(act, nn.SiLU):
+        return type(act).forward is nn.SiLU.forward
+    return isinstance(act, nn.Module) and type(act).__name__ == "SiLUActivation"
+
+
+def _unhooked(m: nn.Module) -> bool:
+    """Calling m is its class's forward and nothing else."""
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
 def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
-    """The dense kernels take device tensors of one dtype and plain nn.Linear modules; anything else (autocast,
-    a projection replaced later, hooks on one) runs the modules' own forward."""
-    for m in (mlp.gate_proj, mlp.up_proj, mlp.down_proj):
-        if type(m) is not nn.Linear or m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
-            return False
+    """The dense kernels take device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
+    (autocast, a projection or the activation replaced later, hooks on one) runs the modules' own forward."""
+    mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
+    if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
+        return False
+    if not all(_unhooked(m) for m in (*mods, mlp.act_fn)):
+        return False
     ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
     return (mlp.gate_proj.bias is None and mlp.up_proj.bias is None and x.is_cuda and x.dtype in _lib.DTYPE_CODE and not torch.is_autocast_enabled("cuda")
             and all(t is None or (t.dtype == x.dtype and t.device == x.device) for t in ws))
@@ -484,8 +498,8 @@ def fuse_dense_mlp(model) -> int:
     up projections with their product in one launch, the down projection in another, in training too
     (bcfft.dense is differentiable in every operand). The rewired forward also takes a residual that the
     down projection adds in its epilogue. Parameters and state_dict are unchanged; an MLP one of whose three
-    modules is replaced afterwards or holds hooks runs the modules' own forward. Returns the number of MLPs
-    rewired."""
+    projections, or whose activation, is replaced afterwards or holds hooks runs the modules' own forward.
+    Returns the number of MLPs rewired."""
     import types
     n = 0
     for layer in model.model.layers:
@@ -493,10 +507,9 @@ def fuse_dense_mlp(model) -> int:
         mods = [getattr(mlp, nm, None) for nm in MLP_PROJECTIONS] if mlp is not None else []
         if len(mods) != 3 or not all(type(m) is nn.Linear for m in mods):
             continue
-        act = getattr(mlp, "act_fn", None)          # nn.SiLU, or transformers' SiLUActivation
         if mods[0].bias is not None or mods[1].bias is not None:
             continue
-        if not (isinstance(act, nn.SiLU) or type(act).__name__ == "SiLUActivation"):
+        if not _plain_silu(getattr(mlp, "act_fn", None)):
             continue
         mlp.forward = types.MethodType(_dense_mlp_forward, mlp)
         n += 1

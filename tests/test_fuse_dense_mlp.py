@@ -1,0 +1,100 @@
+"""Which path a rewired dense MLP takes (patch_llama_fft.fuse_dense_mlp), on the CPU: FakeTensors on a ROCm
+device, so no launch, and the two operators replaced by recorders."""
+import types
+
+import pytest
+import torch
+import torch.nn as nn
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import patch_llama_fft as P
+
+HIDDEN, INNER = 32, 48
+
+
+class MLP(nn.Module):
+    def __init__(self, act=None, device="cuda", dtype=torch.bfloat16):
+        super().__init__()
+        kw = dict(bias=False, device=device, dtype=dtype)
+        self.gate_proj, self.up_proj = nn.Linear(HIDDEN, INNER, **kw), nn.Linear(HIDDEN, INNER, **kw)
+        self.down_proj = nn.Linear(INNER, HIDDEN, **kw)
+        self.act_fn = nn.SiLU() if act is None else act
+
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+def model_of(*mlps):
+    return types.SimpleNamespace(model=types.SimpleNamespace(layers=[types.SimpleNamespace(mlp=m) for m in mlps]))
+
+
+@pytest.fixture
+def fused_calls(monkeypatch):
+    """The calls of the dense operators, which stand in by their shapes."""
+    calls = []
+
+    def glu(x, w_gate, w_up, *, activation="silu"):
+        calls.append("glu")
+        return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
+
+    def linear(x, weight, bias=None, *, activation=None, residual=None):
+        calls.append("linear")
+        return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+    monkeypatch.setattr(P, "_dense", types.SimpleNamespace(glu=glu, linear=linear))
+    return calls
+
+
+@pytest.fixture
+def fake():
+    with FakeTensorMode() as mode, torch.no_grad():
+        yield mode
+
+
+def rewired():
+    mlp = MLP()
+    assert P.fuse_dense_mlp(model_of(mlp)) == 1
+    return mlp, torch.empty(2, 3, HIDDEN, device="cuda", dtype=torch.bfloat16)
+
+
+def test_plain_modules_run_fused(fake, fused_calls):
+    mlp, x = rewired()
+    assert mlp(x).shape == x.shape and fused_calls == ["glu", "linear"]
+
+
+def test_replaced_activation_runs_the_modules(fake, fused_calls):
+    """An activation replaced after the call is the one that is computed."""
+    mlp, x = rewired()
+    seen = []
+
+    class Watched(nn.GELU):
+        def forward(self, z):
+            seen.append(tuple(z.shape))
+            return super().forward(z)
+
+    class Scaled(nn.SiLU):
+        def forward(self, z):
+            seen.append(tuple(z.shape))
+            return 2 * super().forward(z)
+
+    for act in (Watched(), Scaled()):
+        mlp.act_fn = act
+        assert mlp(x).shape == x.shape
+        assert fused_calls == [] and seen.pop() == (2, 3, INNER)
+    mlp.act_fn = nn.SiLU()
+    mlp(x)
+    assert fused_calls == ["glu", "linear"]
+    assert P.fuse_dense_mlp(model_of(MLP(act=Scaled()))) == 0
+
+
+def test_hooked_activation_is_called(fake, fused_calls):
+    mlp, x = rewired()
+    seen = []
+    for register in (mlp.act_fn.register_forward_hook, mlp.act_fn.register_forward_pre_hook):
+        handle = register(lambda *a: seen.append(len(a)))
+        mlp(x)
+        assert len(seen) == 1 and fused_calls == []
+        handle.remove()
+        seen.clear()
+    mlp(x)
+    assert fused_calls == ["glu", "linear"]
