@@ -465,18 +465,20 @@ def _plain_silu(act) -> bool:
     return isinstance(act, nn.Module) and type(act).__name__ == "SiLUActivation"
 
 
-def _unhooked(m: nn.Module) -> bool:
-    """Calling m is its class's forward and nothing else."""
-    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+def _as_its_class(m: nn.Module) -> bool:
+    """Calling m is its class's forward and nothing else: no hooks, no forward of the instance's own (as
+    offloading wrappers and this file's rewirings set it)."""
+    return "forward" not in m.__dict__ and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or
+                                                m._backward_pre_hooks)
 
 
 def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
     """The dense kernels take device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
-    (autocast, a projection or the activation replaced later, hooks on one) runs the modules' own forward."""
+    (autocast, a projection or the activation replaced later, hooks or a forward set on one) runs the modules' own forward."""
     mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
     if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
         return False
-    if not all(_unhooked(m) for m in (*mods, mlp.act_fn)):
+    if not all(_as_its_class(m) for m in (*mods, mlp.act_fn)):
         return False
     ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
     return (mlp.gate_proj.bias is None and mlp.up_proj.bias is None and x.is_cuda and x.dtype in _lib.DTYPE_CODE and not torch.is_autocast_enabled("cuda")
@@ -498,8 +500,8 @@ def fuse_dense_mlp(model) -> int:
     up projections with their product in one launch, the down projection in another, in training too
     (bcfft.dense is differentiable in every operand). The rewired forward also takes a residual that the
     down projection adds in its epilogue. Parameters and state_dict are unchanged; an MLP one of whose three
-    projections, or whose activation, is replaced afterwards or holds hooks runs the modules' own forward.
-    Returns the number of MLPs rewired."""
+    projections, or whose activation, is replaced afterwards, holds hooks or a forward of its own runs as the
+    modules that they are. Returns the number of MLPs rewired."""
     import types
     n = 0
     for layer in model.model.layers:

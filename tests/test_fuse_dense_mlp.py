@@ -98,3 +98,22 @@ def test_hooked_activation_is_called(fake, fused_calls):
         seen.clear()
     mlp(x)
     assert fused_calls == ["glu", "linear"]
+
+
+@pytest.mark.parametrize("name", ["gate_proj", "up_proj", "down_proj", "act_fn"])
+def test_replaced_instance_forward_is_called(fake, fused_calls, name):
+    """m.forward = ..., as offloading wrappers set it: the module's class stays what it was."""
+    mlp, x = rewired()
+    m = getattr(mlp, name)
+    own, seen = m.forward, []
+
+    def wrapper(z):
+        seen.append(name)
+        return own(z)
+
+    m.forward = wrapper
+    assert mlp(x).shape == x.shape
+    assert seen == [name] and fused_calls == []
+    del m.forward
+    mlp(x)
+    assert fused_calls == ["glu", "linear"]
