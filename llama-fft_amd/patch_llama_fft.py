@@ -472,13 +472,20 @@ def _as_its_class(m: nn.Module) -> bool:
                                                 m._backward_pre_hooks)
 
 
+def _hooks_on_every_module() -> bool:
+    """torch.nn.modules.module.register_module_*_hook: they fire for the projections and the activation too."""
+    m = nn.modules.module
+    return bool(m._global_forward_hooks or m._global_forward_pre_hooks or m._global_backward_hooks or
+                m._global_backward_pre_hooks)
+
+
 def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
     """The dense kernels take device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
     (autocast, a projection or the activation replaced later, hooks or a forward set on one) runs the modules' own forward."""
     mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
     if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
         return False
-    if not all(_as_its_class(m) for m in (*mods, mlp.act_fn)):
+    if not all(_as_its_class(m) for m in (*mods, mlp.act_fn)) or _hooks_on_every_module():
         return False
     ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
     return (mlp.gate_proj.bias is None and mlp.up_proj.bias is None and x.is_cuda and x.dtype in _lib.DTYPE_CODE and not torch.is_autocast_enabled("cuda")

@@ -117,3 +117,21 @@ def test_replaced_instance_forward_is_called(fake, fused_calls, name):
     del m.forward
     mlp(x)
     assert fused_calls == ["glu", "linear"]
+
+
+@pytest.mark.parametrize("register", [
+    torch.nn.modules.module.register_module_forward_hook,
+    torch.nn.modules.module.register_module_forward_pre_hook,
+    torch.nn.modules.module.register_module_full_backward_hook,
+    torch.nn.modules.module.register_module_full_backward_pre_hook])
+def test_hooks_on_every_module_run_the_modules(fake, fused_calls, register):
+    """torch's global module hooks fire for the projections too."""
+    mlp, x = rewired()
+    handle = register(lambda m, *a: None)
+    try:
+        mlp(x)
+        assert fused_calls == []
+    finally:
+        handle.remove()
+    mlp(x)
+    assert fused_calls == ["glu", "linear"]
