@@ -479,17 +479,28 @@ def _hooks_on_every_module() -> bool:
                 m._global_backward_pre_hooks)
 
 
+def _plain_tensor(t: torch.Tensor) -> bool:
+    """Memory that a kernel can read, or a traced stand-in for it: a subclass (sharded, quantised) computes its
+    products itself."""
+    return type(t) in (torch.Tensor, nn.Parameter, torch._subclasses.FakeTensor)
+
+
 def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
-    """The dense kernels take device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
-    (autocast, a projection or the activation replaced later, hooks or a forward set on one) runs the modules' own forward."""
+    """The dense kernels take plain device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
+    (autocast, tensor subclasses, a projection or the activation replaced later, hooks or a forward set on one)
+    runs the modules' own forward."""
     mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
     if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
         return False
     if not all(_as_its_class(m) for m in (*mods, mlp.act_fn)) or _hooks_on_every_module():
         return False
+    if mlp.gate_proj.bias is not None or mlp.up_proj.bias is not None or torch.is_autocast_enabled("cuda"):
+        return False
+    if not x.is_cuda or x.dtype not in _lib.DTYPE_CODE:
+        return False
     ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
-    return (mlp.gate_proj.bias is None and mlp.up_proj.bias is None and x.is_cuda and x.dtype in _lib.DTYPE_CODE and not torch.is_autocast_enabled("cuda")
-            and all(t is None or (t.dtype == x.dtype and t.device == x.device) for t in ws))
+    return _plain_tensor(x) and all(t is None or (_plain_tensor(t) and t.dtype == x.dtype and t.device == x.device)
+                                    for t in ws)
 
 
 def _dense_mlp_forward(self, x, residual=None):

@@ -135,3 +135,43 @@ def test_hooks_on_every_module_run_the_modules(fake, fused_calls, register):
         handle.remove()
     mlp(x)
     assert fused_calls == ["glu", "linear"]
+
+
+class Sharded(torch.Tensor):
+    """A tensor of a kind of its own, as sharded and quantised weights are: it says that it is on the GPU, holds
+    no memory there, and computes its products itself (here by a fake twin)."""
+    @staticmethod
+    def __new__(cls, twin):
+        t = torch.Tensor._make_wrapper_subclass(cls, twin.shape, dtype=twin.dtype, device=twin.device)
+        t.twin = twin
+        return t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        if func is torch.ops.aten.detach.default:
+            return cls(args[0].twin)
+        flat, spec = torch.utils._pytree.tree_flatten((args, kwargs or {}))
+        args, kwargs = torch.utils._pytree.tree_unflatten([t.twin if isinstance(t, Sharded) else t for t in flat], spec)
+        cls.seen.append(func)
+        return func(*args, **kwargs)
+
+    __torch_function__ = torch._C._disabled_torch_function_impl
+
+
+@pytest.mark.parametrize("where", ["gate_proj", "up_proj", "down_proj", "bias", "x"])
+def test_tensor_subclasses_run_the_modules(fused_calls, where):
+    with torch.no_grad(), FakeTensorMode():
+        mlp, x = rewired()
+    Sharded.seen = []
+    if where == "bias":
+        with FakeTensorMode():
+            twin = torch.empty(HIDDEN, device="cuda", dtype=torch.bfloat16)
+        mlp.down_proj.bias = nn.Parameter(Sharded(twin), requires_grad=False)
+    elif where == "x":
+        x = Sharded(x)
+    else:
+        m = getattr(mlp, where)
+        m.weight = nn.Parameter(Sharded(m.weight.detach()), requires_grad=False)
+    with torch.no_grad():
+        assert mlp(x).shape == x.shape
+    assert fused_calls == [] and len(Sharded.seen) >= 1
