@@ -164,7 +164,7 @@ def test_tensor_subclasses_run_the_modules(fused_calls, where):
         mlp, x = rewired()
     Sharded.seen = []
     if where == "bias":
-        with FakeTensorMode():
+        with x.fake_mode:
             twin = torch.empty(HIDDEN, device="cuda", dtype=torch.bfloat16)
         mlp.down_proj.bias = nn.Parameter(Sharded(twin), requires_grad=False)
     elif where == "x":
