@@ -485,10 +485,19 @@ def _plain_tensor(t: torch.Tensor) -> bool:
     return type(t) in (torch.Tensor, nn.Parameter, torch._subclasses.FakeTensor)
 
 
+def _traced_gradient(*ts: torch.Tensor | None) -> bool:
+    """A gradient is recorded while a tracer watches (torch.compile, FakeTensors, make_fx, any dispatch mode):
+    the dense operators' autograd nodes launch kernels, which a trace does not hold."""
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)):
+        return False
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or any(type(t) is torch._subclasses.FakeTensor for t in ts))
+
+
 def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
     """The dense kernels take plain device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
-    (autocast, tensor subclasses, a projection or the activation replaced later, hooks or a forward set on one)
-    runs the modules' own forward."""
+    (autocast, tensor subclasses, a traced training step, a projection or the activation replaced later, hooks or
+    a forward set on one) runs the modules' own forward."""
     mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
     if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
         return False
@@ -499,6 +508,8 @@ def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
     if not x.is_cuda or x.dtype not in _lib.DTYPE_CODE:
         return False
     ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
+    if _traced_gradient(x, *ws):
+        return False
     return _plain_tensor(x) and all(t is None or (_plain_tensor(t) and t.dtype == x.dtype and t.device == x.device)
                                     for t in ws)
 
@@ -516,10 +527,11 @@ def fuse_dense_mlp(model) -> int:
     """Route the MLPs that a patch leaves dense (nn.Linear gate_proj / up_proj without bias, act = SiLU;
     31 of 32 layers with the reference's default NUM_LAYERS_TO_PATCH) through the dense kernels: the gate and
     up projections with their product in one launch, the down projection in another, in training too
-    (bcfft.dense is differentiable in every operand). The rewired forward also takes a residual that the
-    down projection adds in its epilogue. Parameters and state_dict are unchanged; an MLP one of whose three
-    projections, or whose activation, is replaced afterwards, holds hooks or a forward of its own runs as the
-    modules that they are. Returns the number of MLPs rewired."""
+    (bcfft.dense is differentiable in every operand; a training step under torch.compile runs the modules).
+    The rewired forward also takes a residual that the down projection adds in its epilogue. Parameters and
+    state_dict are unchanged; an MLP one of whose three projections, or whose activation, is replaced
+    afterwards, holds hooks or a forward of its own runs as the modules that they are. Returns the number of
+    MLPs rewired."""
     import types
     n = 0
     for layer in model.model.layers:

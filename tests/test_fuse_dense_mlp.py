@@ -175,3 +175,32 @@ def test_tensor_subclasses_run_the_modules(fused_calls, where):
     with torch.no_grad():
         assert mlp(x).shape == x.shape
     assert fused_calls == [] and len(Sharded.seen) >= 1
+
+
+def test_traced_gradients_run_the_modules(fused_calls, monkeypatch):
+    """The operators record no gradient of a traced call (torch.compile, FakeTensors, make_fx, a mode that
+    watches every operation): the modules do. Without a gradient the operators themselves are traced."""
+    with FakeTensorMode() as mode:
+        mlp, x = rewired()
+        mlp(x)
+        assert fused_calls == []
+        with torch.no_grad():
+            mlp(x)
+        assert fused_calls == ["glu", "linear"]
+        for p in mlp.parameters():
+            p.requires_grad_(False)
+        mlp(x)
+        assert fused_calls == ["glu", "linear"] * 2
+        mlp(x.requires_grad_())
+        assert fused_calls == ["glu", "linear"] * 2
+
+    # the same decision for memory that is there, by the state of the tracer alone
+    real = torch.empty(2, requires_grad=True)
+    assert not P._traced_gradient(real)
+    with monkeypatch.context() as mp:
+        mp.setattr(torch.compiler, "is_compiling", lambda: True)
+        assert P._traced_gradient(real) and not P._traced_gradient(real.detach())
+    with mode:
+        assert P._traced_gradient(real)
+        with torch.no_grad():
+            assert not P._traced_gradient(real)
