@@ -494,10 +494,19 @@ def _traced_gradient(*ts: torch.Tensor | None) -> bool:
             or any(type(t) is torch._subclasses.FakeTensor for t in ts))
 
 
+def _dense_mlp_sizes_ok(mlp, x: torch.Tensor) -> bool:
+    """What bcfft.dense serves; a projection of other sizes than x's or than its neighbour's is its modules' to refuse."""
+    inner, hidden = mlp.gate_proj.weight.shape
+    return (mlp.up_proj.weight.shape == (inner, hidden) and x.dim() >= 1 and x.shape[-1] == hidden
+            and 1 <= hidden <= _dense.MAX_FEATURES and 1 <= inner <= _dense.MAX_FEATURES // 2
+            and mlp.down_proj.weight.shape[1] == inner and 1 <= mlp.down_proj.weight.shape[0] <= _dense.MAX_FEATURES
+            and x.numel() // hidden <= _dense.MAX_TOKENS)
+
+
 def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
     """The dense kernels take plain device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
-    (autocast, tensor subclasses, a traced training step, a projection or the activation replaced later, hooks or
-    a forward set on one) runs the modules' own forward."""
+    (autocast, tensor subclasses, a traced training step, sizes past the kernels', a projection or the activation
+    replaced later, hooks or a forward set on one) runs the modules' own forward."""
     mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
     if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
         return False
@@ -505,7 +514,7 @@ def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
         return False
     if mlp.gate_proj.bias is not None or mlp.up_proj.bias is not None or torch.is_autocast_enabled("cuda"):
         return False
-    if not x.is_cuda or x.dtype not in _lib.DTYPE_CODE:
+    if not x.is_cuda or x.dtype not in _lib.DTYPE_CODE or not _dense_mlp_sizes_ok(mlp, x):
         return False
     ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
     if _traced_gradient(x, *ws):

@@ -31,6 +31,7 @@ def model_of(*mlps):
 @pytest.fixture
 def fused_calls(monkeypatch):
     """The calls of the dense operators, which stand in by their shapes."""
+    from bcfft import dense
     calls = []
 
     def glu(x, w_gate, w_up, *, activation="silu"):
@@ -41,7 +42,8 @@ def fused_calls(monkeypatch):
         calls.append("linear")
         return x.new_empty((*x.shape[:-1], weight.shape[0]))
 
-    monkeypatch.setattr(P, "_dense", types.SimpleNamespace(glu=glu, linear=linear))
+    monkeypatch.setattr(P, "_dense", types.SimpleNamespace(
+        glu=glu, linear=linear, MAX_FEATURES=dense.MAX_FEATURES, MAX_TOKENS=dense.MAX_TOKENS))
     return calls
 
 
@@ -204,3 +206,22 @@ def test_traced_gradients_run_the_modules(fused_calls, monkeypatch):
         assert P._traced_gradient(real)
         with torch.no_grad():
             assert not P._traced_gradient(real)
+
+
+def test_sizes_past_the_operators_run_the_modules(fake, fused_calls):
+    from bcfft import dense
+    mlp, _ = rewired()
+    for rows, calls in ((dense.MAX_TOKENS, 2), (dense.MAX_TOKENS + 1, 0), (0, 2)):
+        x = torch.empty(rows, HIDDEN, device="cuda", dtype=torch.bfloat16)
+        assert mlp(x).shape == x.shape and len(fused_calls) == calls
+        fused_calls.clear()
+    for hidden, inner, calls in ((dense.MAX_FEATURES, INNER, 2), (dense.MAX_FEATURES + 1, INNER, 0),
+                                 (HIDDEN, dense.MAX_FEATURES // 2, 2), (HIDDEN, dense.MAX_FEATURES // 2 + 1, 0),
+                                 (0, INNER, 0), (HIDDEN, 0, 0)):
+        mlp = MLP()
+        for name, shape in (("gate_proj", (inner, hidden)), ("up_proj", (inner, hidden)), ("down_proj", (hidden, inner))):
+            getattr(mlp, name).weight = nn.Parameter(torch.empty(shape, device="cuda", dtype=torch.bfloat16))
+        assert P.fuse_dense_mlp(model_of(mlp)) == 1
+        x = torch.empty(3, hidden, device="cuda", dtype=torch.bfloat16)
+        assert mlp(x).shape == x.shape and len(fused_calls) == calls
+        fused_calls.clear()
