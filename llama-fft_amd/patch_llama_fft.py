@@ -503,10 +503,10 @@ def _dense_mlp_sizes_ok(mlp, x: torch.Tensor) -> bool:
             and x.numel() // hidden <= _dense.MAX_TOKENS)
 
 
-def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
+def _dense_mlp_ok(mlp, x: torch.Tensor, residual: torch.Tensor | None) -> bool:
     """The dense kernels take plain device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
-    (autocast, tensor subclasses, a traced training step, sizes past the kernels', a projection or the activation
-    replaced later, hooks or a forward set on one) runs the modules' own forward."""
+    (autocast, tensor subclasses, a traced training step, sizes past the kernels', a residual that broadcasts, a
+    projection or the activation replaced later, hooks or a forward set on one) runs the modules' own forward."""
     mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
     if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
         return False
@@ -516,16 +516,16 @@ def _dense_mlp_ok(mlp, x: torch.Tensor) -> bool:
         return False
     if not x.is_cuda or x.dtype not in _lib.DTYPE_CODE or not _dense_mlp_sizes_ok(mlp, x):
         return False
-    ws = (mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias)
-    if _traced_gradient(x, *ws):
+    if residual is not None and residual.shape != (*x.shape[:-1], mlp.down_proj.weight.shape[0]):
         return False
-    return _plain_tensor(x) and all(t is None or (_plain_tensor(t) and t.dtype == x.dtype and t.device == x.device)
-                                    for t in ws)
+    ts = (x, mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias, residual)
+    return not _traced_gradient(*ts) and all(
+        t is None or (_plain_tensor(t) and t.dtype == x.dtype and t.device == x.device) for t in ts)
 
 
 def _dense_mlp_forward(self, x, residual=None):
     """down(silu(gate(x)) * up(x)) (+ residual, in the down projection's epilogue) in two launches."""
-    if not _dense_mlp_ok(self, x):
+    if not _dense_mlp_ok(self, x, residual):
         y = self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
         return y if residual is None else y + residual
     h = _dense.glu(x, self.gate_proj.weight, self.up_proj.weight, activation="silu")

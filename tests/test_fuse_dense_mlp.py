@@ -225,3 +225,22 @@ def test_sizes_past_the_operators_run_the_modules(fake, fused_calls):
         x = torch.empty(3, hidden, device="cuda", dtype=torch.bfloat16)
         assert mlp(x).shape == x.shape and len(fused_calls) == calls
         fused_calls.clear()
+
+
+def test_residuals_that_the_epilogue_does_not_add(fake, fused_calls):
+    """Of another dtype, a shape that broadcasts, a subclass, or with a traced gradient: added after the modules."""
+    mlp, x = rewired()
+    assert mlp(x, residual=torch.empty_like(x)).dtype == x.dtype and fused_calls == ["glu", "linear"]
+    fused_calls.clear()
+    y = mlp(x, residual=torch.empty(2, 3, HIDDEN, device="cuda"))
+    assert y.dtype == torch.float32 and y.shape == x.shape
+    assert mlp(x, residual=torch.empty(HIDDEN, device="cuda", dtype=x.dtype)).shape == x.shape
+    assert mlp(x, residual=torch.empty(4, 2, 3, HIDDEN, device="cuda", dtype=x.dtype)).shape == (4, 2, 3, HIDDEN)
+    Sharded.seen = []
+    mlp(x, residual=Sharded(x))
+    assert fused_calls == [] and len(Sharded.seen) == 1
+    for p in mlp.parameters():
+        p.requires_grad_(False)
+    with torch.enable_grad():
+        mlp(x, residual=torch.empty_like(x).requires_grad_())
+    assert fused_calls == []
