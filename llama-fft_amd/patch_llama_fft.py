@@ -539,8 +539,8 @@ def fuse_dense_mlp(model) -> int:
     (bcfft.dense is differentiable in every operand; a training step under torch.compile runs the modules).
     The rewired forward also takes a residual that the down projection adds in its epilogue. Parameters and
     state_dict are unchanged; an MLP one of whose three projections, or whose activation, is replaced
-    afterwards, holds hooks or a forward of its own runs as the modules that they are. Returns the number of
-    MLPs rewired."""
+    afterwards, holds hooks or a forward of its own runs as the modules that they are; an MLP whose instance
+    already has a forward of another origin is left alone. Returns the number of MLPs rewired."""
     import types
     n = 0
     for layer in model.model.layers:
@@ -551,6 +551,9 @@ def fuse_dense_mlp(model) -> int:
         if mods[0].bias is not None or mods[1].bias is not None:
             continue
         if not _plain_silu(getattr(mlp, "act_fn", None)):
+            continue
+        forward = mlp.__dict__.get("forward")       # a wrapper around the MLP stays; this file's rewirings do not
+        if forward is not None and getattr(forward, "__func__", None) not in (_dense_mlp_forward, _fused_mlp_forward):
             continue
         mlp.forward = types.MethodType(_dense_mlp_forward, mlp)
         n += 1

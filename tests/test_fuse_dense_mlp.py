@@ -244,3 +244,21 @@ def test_residuals_that_the_epilogue_does_not_add(fake, fused_calls):
     with torch.enable_grad():
         mlp(x, residual=torch.empty_like(x).requires_grad_())
     assert fused_calls == []
+
+
+def test_an_mlp_with_a_forward_of_its_own_is_left_alone(fake, fused_calls):
+    """An offloading wrapper around the whole MLP stays; the rewiring itself can be repeated."""
+    mlp = MLP()
+    own, seen = mlp.forward, []
+
+    def wrapper(x):
+        seen.append(1)
+        return own(x)
+
+    mlp.forward = wrapper
+    assert P.fuse_dense_mlp(model_of(mlp, MLP())) == 1
+    x = torch.empty(2, 3, HIDDEN, device="cuda", dtype=torch.bfloat16)
+    mlp(x)
+    assert seen == [1] and fused_calls == []
+    again, _ = rewired()
+    assert P.fuse_dense_mlp(model_of(again)) == 1
