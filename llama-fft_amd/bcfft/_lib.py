@@ -12,6 +12,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("BCFFT_LIB_PATH") or os.path.join(os.path.dirname(_HERE), "lib", "libbcfft.so")
@@ -200,6 +201,13 @@ def device_guard(device: torch.device):
     if device.index is None or device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+def refuse_forward_mode(what: str, *operands: torch.Tensor | None) -> None:
+    """A dual tensor's tangent would be dropped, and its absence read as a zero derivative."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands):
+        raise RuntimeError(f"{what}: no forward-mode derivatives (an operand is a dual tensor)")
 
 
 def require_device(t: torch.Tensor, what: str) -> None:

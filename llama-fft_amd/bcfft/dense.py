@@ -12,6 +12,7 @@ current stream of x's device and does not synchronise. There is no CPU path: a h
 RuntimeError. To capture a training step into a graph, capture forward and backward together, with no eager
 graph of the same parameters alive. A call that records a gradient runs eagerly (under torch.compile, in a
 torch.compiler.disable region); torch.ops.bcfft.dense_linear / dense_glu carry the forward through a trace.
+Dual tensors (forward-mode differentiation) are refused.
 """
 from __future__ import annotations
 
@@ -158,6 +159,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     dtype before the two products that read it; bias gradients sum the unrounded values."""
     if _lib.native_op():                         # the same call as one C++ op (csrc/bcfft_torch_ops.cpp)
         return _lib.NATIVE_OPS["dense_linear"](x, weight, bias, residual, _activation("bcfft.dense.linear", activation))
+    _lib.refuse_forward_mode("bcfft.dense.linear", x, weight, bias, residual)
     lead = x.shape[:-1]
     act = _check("bcfft.dense.linear", x, [("weight", weight)],
                  [("bias", bias, weight.shape[:1]), ("residual", residual, lead + weight.shape[:1])], activation)
@@ -228,6 +230,7 @@ def glu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation
     backward rounds dg and du once to the dtype before the products that read them."""
     if _lib.native_op():
         return _lib.NATIVE_OPS["dense_glu"](x, w_gate, w_up, _activation("bcfft.dense.glu", activation))
+    _lib.refuse_forward_mode("bcfft.dense.glu", x, w_gate, w_up)
     act = _check("bcfft.dense.glu", x, [("w_gate", w_gate), ("w_up", w_up)], [], activation)
     if 2 * w_gate.shape[0] > MAX_FEATURES:
         raise ValueError(f"bcfft.dense.glu: out_features = {w_gate.shape[0]}, at most {MAX_FEATURES // 2}")

@@ -10,7 +10,7 @@ outside them, and the loss and its gradient are one HIP kernel each over the stu
     loss, dlogits = topk_kl_grad(student_logits, values, indices, rest=rest, temperature=T)
 
 Every function enqueues on the current stream of the logits' device and does not synchronise. There is no
-CPU path: a host tensor raises RuntimeError.
+CPU path: a host tensor raises RuntimeError. Dual tensors (forward-mode differentiation) are refused.
 """
 from __future__ import annotations
 
@@ -60,6 +60,7 @@ def topk_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     if _lib.native_op():                         # the same call as one C++ op (csrc/bcfft_torch_ops.cpp)
         return _lib.NATIVE_OPS["topk_logits"](logits, k, temperature)
     what = "bcfft.distill.topk_logits"
+    _lib.refuse_forward_mode(what, logits)
     _lib.require_device(logits, what)
     x = _rows(logits.detach(), what)
     n, v = x.shape
@@ -81,6 +82,7 @@ class _Operands:
     """The checked, flattened operands of one loss call, and its two launches."""
 
     def __init__(self, logits, values, indices, rest, weight, temperature, what):
+        _lib.refuse_forward_mode(what, logits, values, rest, weight)
         _lib.require_device(logits, what)
         self.x = _rows(logits.detach(), what)
         self.n, self.v = self.x.shape
@@ -178,6 +180,7 @@ def topk_kl(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, *
     if _lib.native_op():
         return _lib.NATIVE_OPS["topk_kl"](logits, values, indices, rest, weight, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
+        _lib.refuse_forward_mode("bcfft.distill.topk_kl", logits, values, rest, weight)
         _lib.require_device(logits, "bcfft.distill.topk_kl")
         return _TopKKL.apply(logits, values, indices, rest, weight, temperature)
     op = _Operands(logits, values, indices, rest, weight, temperature, "bcfft.distill.topk_kl")

@@ -62,6 +62,13 @@ void require_memory(const Tensor& t, const char* what) {
               ": records no gradient of a traced tensor (FakeTensor, torch.compile); run this call eagerly, e.g. under "
               "torch.compiler.disable");
 }
+// forward mode: below autograd a tangent would be dropped, and its absence read as a zero derivative
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <class... T>
+void refuse_forward_mode(const char* what, const T&... operands) {
+  TORCH_CHECK(!(has_tangent(operands) || ...), what, ": no forward-mode derivatives (an operand is a dual tensor)");
+}
 // as torch.autograd.function.once_differentiable: a second differentiation raises instead of missing terms
 variable_list once(variable_list out, const Tensor& upstream) {
   if (!(at::GradMode::is_enabled() && wants_grad(upstream))) return out;
@@ -254,6 +261,7 @@ struct GluFn : torch::autograd::Function<GluFn> {
 
 // ------------------------------------------------------------------ distillation from top logits
 constexpr int64_t MAX_ENTRIES = 1024, MAX_VOCAB = 1 << 18;
+constexpr const char *TOPK = "bcfft.distill.topk_logits", *KL = "bcfft.distill.topk_kl", *KL_GRAD = "bcfft.distill.topk_kl_grad";
 
 Tensor logit_rows(const Tensor& logits, const char* what) {
   require_device(logits, what);
@@ -270,7 +278,7 @@ void check_temperature(double t, const char* what) {
 }
 
 std::tuple<Tensor, Tensor, Tensor> topk_run(const Tensor& logits, int64_t k, double temperature) {
-  constexpr const char* what = "bcfft.distill.topk_logits";
+  const char* const what = TOPK;
   const Tensor x = logit_rows(logits, what);
   const int64_t n = x.size(0), v = x.size(1);
   TORCH_CHECK_VALUE(k >= 1 && k <= std::min(v, MAX_ENTRIES), what, ": k = ", k, " must lie in [1, min(vocabulary = ", v,
@@ -343,7 +351,6 @@ std::tuple<Tensor, Tensor, Tensor> kl_run(const Tensor& logits, const KlOperands
   return {loss, st, g};
 }
 
-constexpr const char* KL = "bcfft.distill.topk_kl";
 struct TopKKlFn : torch::autograd::Function<TopKKlFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& values, const Tensor& indices,
                         const OptTensor& rest, const OptTensor& weight, double temperature) {
@@ -388,8 +395,7 @@ Tensor topk_kl_hip(const Tensor& logits, const Tensor& values, const Tensor& ind
 }
 std::tuple<Tensor, Tensor> topk_kl_grad_hip(const Tensor& logits, const Tensor& values, const Tensor& indices,
                                             const OptTensor& rest, const OptTensor& weight, double temperature) {
-  auto [loss, stats, grad] = kl_run(
-      logits, kl_operands(logits, values, indices, rest, weight, temperature, "bcfft.distill.topk_kl_grad"), false, true);
+  auto [loss, stats, grad] = kl_run(logits, kl_operands(logits, values, indices, rest, weight, temperature, KL_GRAD), false, true);
   return {loss, grad};
 }
 
@@ -424,6 +430,7 @@ auto below(const char* name, F) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<std::remove_pointer_t<F>>();
 }
 Tensor dense_linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t act) {
+  refuse_forward_mode(LINEAR, x, weight, bias, residual);
   if (at::GradMode::is_enabled() && !x.is_meta()) {
     const bool inner = wants_grad(x) || wants_grad(weight) || wants_grad(bias);
     if (inner || wants_grad(residual)) {
@@ -436,6 +443,7 @@ Tensor dense_linear_autograd(const Tensor& x, const Tensor& weight, const OptTen
   return op.call(x, weight, bias, residual, act);
 }
 Tensor dense_glu_autograd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int64_t act) {
+  refuse_forward_mode(GLU, x, w_gate, w_up);
   if (at::GradMode::is_enabled() && !x.is_meta() && (wants_grad(x) || wants_grad(w_gate) || wants_grad(w_up))) {
     require_memory(x, GLU);
     return GluFn::apply(x, w_gate, w_up, act);
@@ -446,6 +454,7 @@ Tensor dense_glu_autograd(const Tensor& x, const Tensor& w_gate, const Tensor& w
 }
 Tensor topk_kl_autograd(const Tensor& logits, const Tensor& values, const Tensor& indices, const OptTensor& rest,
                         const OptTensor& weight, double temperature) {
+  refuse_forward_mode(KL, logits, values, rest, weight);
   if (at::GradMode::is_enabled() && !logits.is_meta() && wants_grad(logits)) {
     require_memory(logits, KL);
     return TopKKlFn::apply(logits, values, indices, rest, weight, temperature);
@@ -456,12 +465,14 @@ Tensor topk_kl_autograd(const Tensor& logits, const Tensor& values, const Tensor
 }
 // no gradient flows through these two: the teacher is a constant, and the second returns its gradient
 std::tuple<Tensor, Tensor, Tensor> topk_logits_autograd(const Tensor& logits, int64_t k, double temperature) {
+  refuse_forward_mode(TOPK, logits);
   at::AutoDispatchBelowADInplaceOrView guard;
   static auto op = below("bcfft_native::topk_logits", &topk_run);
   return op.call(logits, k, temperature);
 }
 std::tuple<Tensor, Tensor> topk_kl_grad_autograd(const Tensor& logits, const Tensor& values, const Tensor& indices,
                                                  const OptTensor& rest, const OptTensor& weight, double temperature) {
+  refuse_forward_mode(KL_GRAD, logits, values, rest, weight);
   at::AutoDispatchBelowADInplaceOrView guard;
   static auto op = below("bcfft_native::topk_kl_grad", &topk_kl_grad_hip);
   return op.call(logits, values, indices, rest, weight, temperature);
