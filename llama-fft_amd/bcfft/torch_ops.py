@@ -91,12 +91,14 @@ def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
                  residual: torch.Tensor | None = None, activation: str = "none") -> torch.Tensor:
     """act(x W^T + bias) + residual: bcfft.dense.linear's forward (the projections that
     patch_llama_fft.py:343-394 leaves dense)."""
+    _lib.refuse_forward_mode("bcfft::dense_linear", x, weight, bias, residual)
     with torch.no_grad():
         return dense.linear(x, weight, bias, activation=None if activation == "none" else activation, residual=residual)
 
 
 @dense_linear.register_fake
 def _dense_linear_fake(x, weight, bias=None, residual=None, activation="none"):
+    _lib.refuse_forward_mode("bcfft::dense_linear", x, weight, bias, residual)
     if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
         raise ValueError("bcfft::dense_linear: weight must be (out_features, in_features)")
     return x.new_empty((*x.shape[:-1], weight.shape[0]))
@@ -105,12 +107,14 @@ def _dense_linear_fake(x, weight, bias=None, residual=None, activation="none"):
 @torch.library.custom_op("bcfft::dense_glu", mutates_args=())
 def dense_glu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """act(x Wg^T) * (x Wu^T): bcfft.dense.glu's forward (the dense MLP's inner product)."""
+    _lib.refuse_forward_mode("bcfft::dense_glu", x, w_gate, w_up)
     with torch.no_grad():
         return dense.glu(x, w_gate, w_up, activation=None if activation == "none" else activation)
 
 
 @dense_glu.register_fake
 def _dense_glu_fake(x, w_gate, w_up, activation="silu"):
+    _lib.refuse_forward_mode("bcfft::dense_glu", x, w_gate, w_up)
     if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape[1] != x.shape[-1] or w_up.shape != w_gate.shape:
         raise ValueError("bcfft::dense_glu: w_gate and w_up must be (out_features, in_features)")
     return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
@@ -119,11 +123,13 @@ def _dense_glu_fake(x, w_gate, w_up, activation="silu"):
 @torch.library.custom_op("bcfft::topk_logits", mutates_args=())
 def topk_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """A teacher's k largest logits, indices and rest: bcfft.distill.topk_logits (calibrate_bc.py:192-212)."""
+    _lib.refuse_forward_mode("bcfft::topk_logits", logits)
     return distill.topk_logits(logits, k, temperature)
 
 
 @topk_logits.register_fake
 def _topk_logits_fake(logits, k, temperature=1.0):
+    _lib.refuse_forward_mode("bcfft::topk_logits", logits)
     if logits.dim() < 1 or not 1 <= k <= logits.shape[-1]:
         raise ValueError("bcfft::topk_logits: logits must be (..., V) with 1 <= k <= V")
     lead = logits.shape[:-1]
@@ -135,11 +141,13 @@ def _topk_logits_fake(logits, k, temperature=1.0):
 def topk_kl(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, rest: torch.Tensor | None = None,
             weight: torch.Tensor | None = None, temperature: float = 1.0) -> torch.Tensor:
     """KL per row from the teacher's top logits: bcfft.distill.topk_kl's forward (calibrate_bc.py:281-294)."""
+    _lib.refuse_forward_mode("bcfft::topk_kl", logits, values, rest, weight)
     return distill.topk_kl(logits.detach(), values, indices, rest=rest, weight=weight, temperature=temperature)
 
 
 @topk_kl.register_fake
 def _topk_kl_fake(logits, values, indices, rest=None, weight=None, temperature=1.0):
+    _lib.refuse_forward_mode("bcfft::topk_kl", logits, values, rest, weight)
     if values.shape != indices.shape or values.shape[:-1] != logits.shape[:-1]:
         raise ValueError("bcfft::topk_kl: values and indices must both be logits' leading shape + (k,)")
     return logits.new_empty(logits.shape[:-1], dtype=torch.float32)
@@ -149,11 +157,13 @@ def _topk_kl_fake(logits, values, indices, rest=None, weight=None, temperature=1
 def topk_kl_grad(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, rest: torch.Tensor | None = None,
                  weight: torch.Tensor | None = None, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """Losses and the gradient of their sum in one launch: bcfft.distill.topk_kl_grad."""
+    _lib.refuse_forward_mode("bcfft::topk_kl_grad", logits, values, rest, weight)
     return distill.topk_kl_grad(logits.detach(), values, indices, rest=rest, weight=weight, temperature=temperature)
 
 
 @topk_kl_grad.register_fake
 def _topk_kl_grad_fake(logits, values, indices, rest=None, weight=None, temperature=1.0):
+    _lib.refuse_forward_mode("bcfft::topk_kl_grad", logits, values, rest, weight)
     return (_topk_kl_fake(logits, values, indices, rest, weight, temperature),
             torch.empty(logits.shape, dtype=logits.dtype, device=logits.device))
 

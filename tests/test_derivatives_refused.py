@@ -77,3 +77,24 @@ def test_functional_jvp_is_refused(path, name):
         return call({**o, duals[0]: t})
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(f, (o[duals[0]],), (torch.ones_like(o[duals[0]]),))
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_registered_operators_refuse_forward_mode(built_lib, name):
+    """torch.ops.bcfft.* (forward only) drop into the operators below autograd: they look at their operands too."""
+    import bcfft.torch_ops  # noqa: F401
+    ops = torch.ops.bcfft
+    calls = {
+        "linear": lambda o: ops.dense_linear(o["x"], o["weight"], o["bias"], o["residual"], "gelu"),
+        "glu": lambda o: ops.dense_glu(o["x"], o["weight"], o["w_up"], "silu"),
+        "topk_kl": lambda o: ops.topk_kl(o["logits"], o["values"], o["indices"], o["rest"], o["w"], 1.0),
+        "topk_kl_grad": lambda o: ops.topk_kl_grad(o["logits"], o["values"], o["indices"], o["rest"], o["w"], 1.0),
+        "topk_logits": lambda o: ops.topk_logits(o["logits"], 3, 1.0),
+    }
+    for device in ("cpu", "meta"):
+        for which in CALLS[name][1]:
+            with fwAD.dual_level():
+                o = operands(device)
+                o[which] = fwAD.make_dual(o[which], torch.ones_like(o[which]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    calls[name](o)
