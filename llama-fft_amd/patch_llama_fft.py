@@ -26,6 +26,7 @@ from typing import Dict
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from bcfft import dense as _dense
@@ -494,6 +495,15 @@ def _traced_gradient(*ts: torch.Tensor | None) -> bool:
             or any(type(t) is torch._subclasses.FakeTensor for t in ts))
 
 
+def _transformed(*ts: torch.Tensor | None) -> bool:
+    """Inside a torch.func transform, or dual tensors: the modules' products have rules for them. (torch.compile
+    traces a transform's body apart from it; its view of the transforms' stack is not this thread's.)"""
+    if not torch.compiler.is_compiling() and torch._C._functorch.peek_interpreter_stack() is not None:
+        return True
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
 def _dense_mlp_sizes_ok(mlp, x: torch.Tensor) -> bool:
     """What bcfft.dense serves; a projection of other sizes than x's or than its neighbour's is its modules' to refuse."""
     inner, hidden = mlp.gate_proj.weight.shape
@@ -505,8 +515,9 @@ def _dense_mlp_sizes_ok(mlp, x: torch.Tensor) -> bool:
 
 def _dense_mlp_ok(mlp, x: torch.Tensor, residual: torch.Tensor | None) -> bool:
     """The dense kernels take plain device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
-    (autocast, tensor subclasses, a traced training step, sizes past the kernels', a residual that broadcasts, a
-    projection or the activation replaced later, hooks or a forward set on one) runs the modules' own forward."""
+    (autocast, tensor subclasses, a traced training step, torch.func transforms and dual tensors, sizes past the
+    kernels', a residual that broadcasts, a projection or the activation replaced later, hooks or a forward set
+    on one) runs the modules' own forward."""
     mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
     if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
         return False
@@ -519,7 +530,7 @@ def _dense_mlp_ok(mlp, x: torch.Tensor, residual: torch.Tensor | None) -> bool:
     if residual is not None and residual.shape != (*x.shape[:-1], mlp.down_proj.weight.shape[0]):
         return False
     ts = (x, mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias, residual)
-    return not _traced_gradient(*ts) and all(
+    return not _traced_gradient(*ts) and not _transformed(*ts) and all(
         t is None or (_plain_tensor(t) and t.dtype == x.dtype and t.device == x.device) for t in ts)
 
 

@@ -262,3 +262,19 @@ def test_an_mlp_with_a_forward_of_its_own_is_left_alone(fake, fused_calls):
     assert seen == [1] and fused_calls == []
     again, _ = rewired()
     assert P.fuse_dense_mlp(model_of(again)) == 1
+
+
+def test_transforms_run_the_modules(fake, fused_calls):
+    """Forward-mode derivatives and torch.func transforms pass through the modules, which have rules for them."""
+    import torch.autograd.forward_ad as fwAD
+    mlp, x = rewired()
+    with fwAD.dual_level():
+        mlp(x)
+        assert fused_calls == ["glu", "linear"]        # a level alone changes nothing
+        y = mlp(fwAD.make_dual(x, torch.ones_like(x)))
+        assert fwAD.unpack_dual(y).tangent.shape == x.shape
+        mlp(x, residual=fwAD.make_dual(x, torch.ones_like(x)))
+    y, t = torch.func.jvp(mlp, (x,), (torch.ones_like(x),))
+    assert t.shape == x.shape
+    assert torch.func.vmap(mlp)(x).shape == x.shape
+    assert fused_calls == ["glu", "linear"]

@@ -62,3 +62,19 @@ def test_compiled_forward_and_training_step(mlp):
     want.backward(dy.double())
     for p, w in zip((mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight), weights):
         close(p.grad, w.grad)
+
+
+def test_transforms_and_forward_mode(mlp):
+    """torch.func.grad, jvp and vmap over a rewired MLP: derivatives of the fp64 formula."""
+    x, t = torch.randn(5, HIDDEN, device="cuda:0"), torch.randn(5, HIDDEN, device="cuda:0")
+    x64 = x.double().requires_grad_()
+    want = plain(mlp, x64)[0]
+    (dx,) = torch.autograd.grad(want.sum(), x64, retain_graph=True)
+    close(torch.func.grad(lambda v: mlp(v).sum())(x), dx)
+    close(torch.func.vmap(mlp)(x), want.detach())
+    for p in mlp.parameters():
+        p.requires_grad_(False)
+    y, jvp = torch.func.jvp(mlp, (x,), (t,))
+    _, want_jvp = torch.autograd.functional.jvp(lambda v: plain(mlp, v)[0], x.double(), t.double())
+    close(y, want.detach())
+    close(jvp, want_jvp)
