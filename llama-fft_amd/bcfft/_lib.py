@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 
@@ -208,6 +209,24 @@ def refuse_forward_mode(what: str, *operands: torch.Tensor | None) -> None:
     if forward_ad._current_level >= 0 and any(
             t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands):
         raise RuntimeError(f"{what}: no forward-mode derivatives (an operand is a dual tensor)")
+
+
+def first_order(backward):
+    """Decorates an autograd Function's backward that has no derivative of its own: where it is recorded
+    (create_graph) a second differentiation raises instead of missing terms, whether or not the incoming gradient
+    needs one (dx depends on w). What passes an incoming gradient on is left as it is."""
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+            out = out if isinstance(out, tuple) else (out,)
+        if not torch.is_grad_enabled():
+            return out
+        fail = torch._C._functions.DelayedError(
+            "trying to differentiate twice a function whose backward is not differentiable", len(out))
+        marked = fail(*[None if t is None else t.detach().requires_grad_() for t in out])
+        return tuple(t if t is None or any(t is g for g in grads) else m for t, m in zip(out, marked))
+    return wrapper
 
 
 def require_device(t: torch.Tensor, what: str) -> None:

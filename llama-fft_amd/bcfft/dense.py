@@ -17,7 +17,6 @@ Dual tensors (forward-mode differentiation) are refused.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -126,7 +125,7 @@ class _Linear(torch.autograd.Function):
         return y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
@@ -200,7 +199,7 @@ class _Glu(torch.autograd.Function):
         return h.view(*x.shape[:-1], wg.shape[0])
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dh):
         x, w_gate, w_up, gu = ctx.saved_tensors
         need_x, need_g, need_u = ctx.needs_input_grad[:3]

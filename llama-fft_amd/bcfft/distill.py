@@ -17,7 +17,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -157,7 +156,7 @@ class _TopKKL(torch.autograd.Function):
         return loss.view(logits.shape[:-1])
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dloss):
         logits, values, indices, rest, weight, stats = ctx.saved_tensors
         op = _Operands(logits, values, indices, rest, weight, ctx.temperature, "bcfft.distill.topk_kl")

@@ -69,14 +69,19 @@ template <class... T>
 void refuse_forward_mode(const char* what, const T&... operands) {
   TORCH_CHECK(!(has_tangent(operands) || ...), what, ": no forward-mode derivatives (an operand is a dual tensor)");
 }
-// as torch.autograd.function.once_differentiable: a second differentiation raises instead of missing terms
-variable_list once(variable_list out, const Tensor& upstream) {
-  if (!(at::GradMode::is_enabled() && wants_grad(upstream))) return out;
+// Where the backward itself is recorded (create_graph), a second differentiation raises instead of missing terms,
+// whether or not the incoming gradient needs one: dx depends on w. What passes the incoming gradient on is left as it is.
+variable_list first_order(variable_list out, const Tensor& upstream) {
+  if (!at::GradMode::is_enabled()) return out;
   auto fail = std::make_shared<torch::autograd::DelayedError>(
-      "trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)out.size());
-  for (Tensor& t : out)
+      "trying to differentiate twice a function whose backward is not differentiable", (int64_t)out.size());
+  variable_list marked(out);
+  for (Tensor& t : marked)
     if (t.defined()) t = t.detach().requires_grad_(true);
-  return (*fail)(std::move(out));
+  marked = (*fail)(std::move(marked));
+  for (size_t i = 0; i < out.size(); ++i)
+    if (out[i].defined() && out[i].is_same(upstream)) marked[i] = out[i];
+  return marked;
 }
 
 // ------------------------------------------------------------------ dense projections
@@ -195,7 +200,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
                      "bcfft_dense_linear_backward");
       }
     }
-    return once({dx, dw, db, need_r ? dy : Tensor(), Tensor(), Tensor()}, dy);
+    return first_order({dx, dw, db, need_r ? dy : Tensor(), Tensor(), Tensor()}, dy);
   }
 };
 
@@ -255,7 +260,7 @@ struct GluFn : torch::autograd::Function<GluFn> {
                      "bcfft_dense_glu_backward");
       }
     }
-    return once({dx, need_g ? dw.select(0, 0) : Tensor(), need_u ? dw.select(0, 1) : Tensor(), Tensor()}, dh);
+    return first_order({dx, need_g ? dw.select(0, 0) : Tensor(), need_u ? dw.select(0, 1) : Tensor(), Tensor()}, dh);
   }
 };
 
@@ -378,7 +383,7 @@ struct TopKKlFn : torch::autograd::Function<TopKKlFn> {
                                                ptr(g), stream_of(o.x)),
                    "bcfft_distill_topk_backward");
     }
-    return once({g, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, grads[0]);
+    return first_order({g, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, grads[0]);
   }
 };
 
