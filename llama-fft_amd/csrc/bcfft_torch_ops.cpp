@@ -6,6 +6,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -55,12 +56,20 @@ int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.siz
 Tensor aligned16(const Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone(at::MemoryFormat::Contiguous) : t;
 }
-// FakeTensors and functionalised tensors have no memory: their shapes come from the Meta kernels, but a C++
-// autograd node here would read them
-void require_memory(const Tensor& t, const char* what) {
-  TORCH_CHECK(!t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python), what,
-              ": records no gradient of a traced tensor (FakeTensor, torch.compile); run this call eagerly, e.g. under "
-              "torch.compiler.disable");
+// FakeTensors, functionalised tensors and other subclasses have no memory to read here, and a trace would not hold
+// the launches of a C++ autograd node: their shapes come from the Meta kernels, below autograd
+bool traced(const Tensor& t) { return t.defined() && t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python); }
+bool traced(const OptTensor& t) { return t.has_value() && traced(*t); }
+template <class... T>
+void require_memory(const char* what, const T&... operands) {
+  using c10::impl::TorchDispatchModeKey, c10::impl::TorchDispatchModeTLS;
+  const bool mode = TorchDispatchModeTLS::any_modes_set() &&
+                    (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) ||
+                     TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) ||
+                     TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL));
+  TORCH_CHECK(!(mode || (traced(operands) || ...)), what,
+              ": records no gradient of a traced tensor (FakeTensor, torch.compile, make_fx, a subclass); run this call "
+              "eagerly, e.g. under torch.compiler.disable");
 }
 // forward mode: below autograd a tangent would be dropped, and its absence read as a zero derivative
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
@@ -439,7 +448,7 @@ Tensor dense_linear_autograd(const Tensor& x, const Tensor& weight, const OptTen
   if (at::GradMode::is_enabled() && !x.is_meta()) {
     const bool inner = wants_grad(x) || wants_grad(weight) || wants_grad(bias);
     if (inner || wants_grad(residual)) {
-      require_memory(x, LINEAR);
+      require_memory(LINEAR, x, weight, bias, residual);
       return LinearFn::apply(x, weight, bias, residual, act, inner && act != BCFFT_ACT_NONE);
     }
   }
@@ -450,7 +459,7 @@ Tensor dense_linear_autograd(const Tensor& x, const Tensor& weight, const OptTen
 Tensor dense_glu_autograd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int64_t act) {
   refuse_forward_mode(GLU, x, w_gate, w_up);
   if (at::GradMode::is_enabled() && !x.is_meta() && (wants_grad(x) || wants_grad(w_gate) || wants_grad(w_up))) {
-    require_memory(x, GLU);
+    require_memory(GLU, x, w_gate, w_up);
     return GluFn::apply(x, w_gate, w_up, act);
   }
   at::AutoDispatchBelowADInplaceOrView guard;
@@ -461,7 +470,7 @@ Tensor topk_kl_autograd(const Tensor& logits, const Tensor& values, const Tensor
                         const OptTensor& weight, double temperature) {
   refuse_forward_mode(KL, logits, values, rest, weight);
   if (at::GradMode::is_enabled() && !logits.is_meta() && wants_grad(logits)) {
-    require_memory(logits, KL);
+    require_memory(KL, logits, values, indices, rest, weight);
     return TopKKlFn::apply(logits, values, indices, rest, weight, temperature);
   }
   at::AutoDispatchBelowADInplaceOrView guard;
