@@ -16,8 +16,9 @@
 // clock (an exponential counts four), so a row's floor allows 14 (28) of them per logit: what the passes
 // cost is counted beside them, and exponentials that the gradient needs again stay in registers.
 //
-// The loss is a small difference of logarithms: a thread's part of a sum is kept in fp32 (at most 128 terms
-// of one sign), the sums over threads, the teacher's softmax and the logarithms in fp64.
+// The loss is a small difference of logarithms: a thread's part of a sum is kept in fp32 for at most 128 terms
+// of one sign and the element behind the last whole piece (longer rows add it to an fp64 sum as often), the sums
+// over threads, the teacher's softmax and the logarithms in fp64.
 #include "bcfft_device.h"
 
 #include <type_traits>
@@ -129,6 +130,28 @@ struct Row {
       f((int)(pieces * VEC) + (int)threadIdx.x, v);
     }
   }
+};
+// One thread's sum over the row, in fp32 with its registers where a row is held. A row that is read again has
+// vocab / 1024 elements per thread (4096 of 2^22 logits: equal terms, whose roundings have one sign, were up to
+// 5e-5 off): every 128 of them go to an fp64 sum.
+template <int HOLD>
+struct ThreadSum {
+  float part = 0.f;
+  double whole = 0.0;
+  int terms = 0;
+  __device__ __forceinline__ void operator+=(float e) { part += e; }
+  template <int N>
+  __device__ __forceinline__ void piece_done() {
+    if constexpr (HOLD == 0) {
+      terms += N;
+      if (terms >= 128) {
+        whole += (double)part;
+        part = 0.f;
+        terms = 0;
+      }
+    }
+  }
+  __device__ __forceinline__ double value() const { return HOLD == 0 ? whole + (double)part : (double)part; }
 };
 template <class A> constexpr int count_of = (int)(sizeof(std::remove_reference_t<A>) / sizeof(float));
 
@@ -295,7 +318,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
   // an element reaches the bound unless it is less: NaN does, and without a bound all do
   const uint32_t bound_key = (uint32_t)bound_s << 16;
   const float bound = bound_key ? key_value(bound_key) : -INFINITY;
-  float s = 0.f;
+  ThreadSum<HOLD> s;
   // one bit per logit of a thread that reaches the bound, listed after the pass: no branch in it
   uint64_t reach = 0;
   int bit = 0, first = tid;              // the next piece's bit, and the piece of bit 0
@@ -318,6 +341,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
         s += under ? exp_near(v[j], es, bound) : 0.f;
         m = m << 1 | (under ? 0 : 1);
       }
+      s.template piece_done<N>();
       if (bit == 0) first = at / VEC;
       reach |= (uint64_t)m << bit;
       bit += N;
@@ -339,7 +363,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
   });
   list();
   // log of the sum of exp(x / T) over the elements under the bound
-  const double sum = block_reduce<NT>((double)s, redd, SumOp());
+  const double sum = block_reduce<NT>(s.value(), redd, SumOp());
   int m = count;
   const bool flood = m > TOPK_CAND;      // uniform over the workgroup, as all that follows from it
   // the mass that is left, as log(under) + ref / T
@@ -387,7 +411,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
     });
     below = block_reduce<NT>(below, redf, MaxOp());
     ref = below == -INFINITY ? 0.f : below;
-    float s2 = 0.f;
+    ThreadSum<HOLD> s2;
     r.each([&](int at, auto& v) {
 #pragma unroll
       for (int j = 0; j < count_of<decltype(v)>; ++j) {
@@ -395,8 +419,9 @@ __global__ __launch_bounds__(NT, NT == 512 ? 6 : 1) void bc_topk_logits_kernel(c
         const bool taken = key > cut_key || (key == cut_key && at <= cut_index - j);
         s2 += taken ? 0.f : exp_at(v[j], es, ref);
       }
+      s2.template piece_done<count_of<decltype(v)>>();
     });
-    under = block_reduce<NT>((double)s2, redd, SumOp());
+    under = block_reduce<NT>(s2.value(), redd, SumOp());
     if (flood) m = k;
   }
 
@@ -655,7 +680,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
     }
   }
   // the other elements' sum
-  float so = 0.f;
+  ThreadSum<HOLD> so;
   float kept[KEEP ? HOLD : 1][VEC], kept_tail = 0.f;
   if constexpr (KEEP) {
 #pragma unroll
@@ -683,9 +708,10 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
       const uint32_t keep = ~piece_bits<N>(bits, at);
 #pragma unroll
       for (int j = 0; j < N; ++j) so += unless(keep, j, exp_at(v[j], a.es, m_all));
+      so.template piece_done<N>();
     });
   }
-  double sums[4] = {(double)so, total, se, lin};
+  double sums[4] = {so.value(), total, se, lin};
 #pragma unroll
   for (int q = 0; q < 4; ++q) sums[q] = wave_reduce(sums[q], SumOp());
   if ((tid & 63) == 0) {
@@ -714,14 +740,15 @@ __global__ __launch_bounds__(NT, NT == 512 ? (GRAD ? 4 : 6) : 1) void bc_distill
     });
     mo = block_reduce<NT>(mo, en.redf, MaxOp());
     ref = mo == -INFINITY ? 0.f : mo;
-    float s2 = 0.f;
+    ThreadSum<HOLD> s2;                  // as many terms per thread as where the row is held
     r2.each([&](int at, auto& v) {
       constexpr int N = count_of<decltype(v)>;
       const uint32_t keep = ~piece_bits<N>(bits, at);
 #pragma unroll
       for (int j = 0; j < N; ++j) s2 += unless(keep, j, exp_at(v[j], a.es, ref));
+      s2.template piece_done<N>();
     });
-    sum_ref = block_reduce<NT>((double)s2, en.topd, SumOp());
+    sum_ref = block_reduce<NT>(s2.value(), en.topd, SumOp());
     sum_o = mo == -INFINITY ? 0.0 : sum_ref * exp(((double)ref - (double)m_all) * a.inv_t);
   }
   const double sum = sum_o + sum_e, inv_s = 1.0 / sum;

@@ -507,3 +507,34 @@ def test_more_rows_than_one_launch(dev):
     loss = distill.topk_kl(sg, values, indices.long(), rest=rest, weight=weight, temperature=t)
     loss.backward(torch.full_like(loss, 3.0))
     check_grad(sg.grad, dwant, size, 3.0)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_many_equal_terms(dev, dt):
+    """Rows that are read again: each thread adds thousands of equal exponentials (of 2.5 under the bound, and of
+    2.5 under the others' own maximum where the bound lies far above), whose roundings all have one sign."""
+    from bcfft import distill
+    v, k = (1 << 22) + 3, 8
+    z = torch.full((2, v), -1.5)
+    z[0, :: v // 40] = 1.0
+    z[1] = -72.5
+    z[1, 5] = -70.0
+    z[1, 1:: v // 40] = 1.0
+    z = z.to(DT[dt])
+    values, indices, rest = distill.topk_logits(z.to(dev), k)
+    top, want = teacher_oracle(z, k, 1.0)
+    assert torch.equal(indices.cpu().long(), top) and torch.equal(values.cpu(), z.gather(-1, top))
+    assert bool(((rest.double().cpu() - want).abs() <= LOG_TOL + 2.0 ** -23 * want.abs()).all())
+    v = 1 << 18
+    s = torch.full((2, v), -2.3)
+    s[0, :: v // 40] = 0.0
+    s[1] = -102.3
+    s[1, 100:110] = -100.0
+    s[1, :4] = 0.0
+    s = s.to(DT[dt])
+    top = torch.tensor([[0, 1, 7], [0, 1, 2]])
+    vals, rest = torch.tensor([[1.0, 0.5, 0.25]]).expand(2, 3).contiguous(), torch.tensor([2.0, 1.0])
+    want, dwant, size = kl_oracle(s, vals, top, rest, None, 1.0)
+    loss, grad = distill.topk_kl_grad(s.to(dev), vals.to(dev), top.to(dev), rest=rest.to(dev))
+    check_loss(loss, want)
+    check_grad(grad, dwant, size)
