@@ -318,6 +318,13 @@ enum bcfft_dense_op { BCFFT_DENSE_LINEAR = 0, BCFFT_DENSE_GLU = 1, BCFFT_DENSE_L
 int64_t bcfft_dense_workspace_bytes(int op, int64_t n_tokens, int64_t in_features, int64_t out_features, int dtype,
                                     int act);
 
+/* How one product of such a call is cut on the current device: *kind, the rows x columns of a workgroup's tile
+ * (0: few rows, or few tokens' weight gradient; 1: 128 x 128; 2: 256 x 128; 3: 256 x 256; 4: 64 x 128; 5: 32 x
+ * 128; 6: 64 x 64), and *slices of k. product: of a forward 0; of a backward 0 the input gradient, 1 the weight
+ * gradient. Which calls run the same kernels, for tests and measurements; n_tokens >= 1. */
+int bcfft_dense_plan(int op, int product, int64_t n_tokens, int64_t in_features, int64_t out_features, int dtype, int* kind,
+                     int* slices);
+
 int bcfft_dense_linear(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
                        int64_t out_features, const void* w, const void* bias, const void* residual, int64_t r_stride,
                        int act, void* y, float* z, void* workspace, int64_t workspace_bytes, void* stream);

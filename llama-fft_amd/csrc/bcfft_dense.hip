@@ -326,6 +326,27 @@ int64_t bcfft_dense_workspace_bytes(int op, int64_t n_tokens, int64_t in_feature
   return backward_plan(n_tokens, in_features, out_features, dtype, parts, act).total;
 }
 
+int bcfft_dense_plan(int op, int product, int64_t n_tokens, int64_t in_features, int64_t out_features, int dtype, int* kind,
+                     int* slices) {
+  const int64_t n = n_tokens, k = in_features, m = out_features;
+  if (!valid_dt(dtype)) return BCFFT_ERR_DTYPE;
+  if (!valid_sizes(n, k, m) || n == 0) return BCFFT_ERR_SHAPE;
+  const bool backward = op == BCFFT_DENSE_LINEAR_BACKWARD || op == BCFFT_DENSE_GLU_BACKWARD;
+  if (op < BCFFT_DENSE_LINEAR || op > BCFFT_DENSE_GLU_BACKWARD || product < 0 || product > (backward ? 1 : 0) || !kind || !slices)
+    return BCFFT_ERR_ARG;
+  const int parts = op == BCFFT_DENSE_GLU || op == BCFFT_DENSE_GLU_BACKWARD ? 2 : 1;
+  Shape sh;
+  if (backward) {
+    const BackwardPlan p = backward_plan(n, k, m, dtype, parts, BCFFT_ACT_NONE);
+    sh = product ? p.dw : p.dx;
+  } else {
+    sh = forward_plan(n, k, m, dtype, parts).shape;
+  }
+  *kind = sh.kind;
+  *slices = sh.kz;
+  return BCFFT_OK;
+}
+
 int bcfft_dense_linear(const void* x, int dtype, int64_t n_tokens, int64_t x_stride, int64_t in_features,
                        int64_t out_features, const void* w, const void* bias, const void* residual, int64_t r_stride,
                        int act, void* y, float* z, void* workspace, int64_t workspace_bytes, void* stream) {
