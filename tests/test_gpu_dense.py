@@ -543,3 +543,31 @@ def test_millions_of_rows(dev, n):
     x, w = rand(dev, n, 7, dt=torch.float16, seed=141), rand(dev, 5, 7, dt=torch.float16, seed=142)
     want = x.double() @ w.double().t()
     within(dense.linear(x, w), want, sum_slack(x.double(), w.double().t()))
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("n,k,m", SIZES)
+def test_relu_gradients(dev, dt, n, k, m):
+    """relu in every size: where rounding may move z across the kink, no gradient comes in (either slope times 0)."""
+    from bcfft import dense
+    x, w, wu = (rand(dev, *s, dt=DT[dt], seed=151 + i, scale=c) for i, (s, c) in
+                enumerate((((n, k), 1.0), ((m, k), k ** -0.5), ((m, k), k ** -0.5))))
+    b, dy = rand(dev, m, dt=DT[dt], seed=155), rand(dev, n, m, dt=DT[dt], seed=156)
+    want, slack, z, zs, slope = linear64(x, w, b, None, "relu")
+    dy0 = torch.where(z.abs() <= zs, torch.zeros_like(dy), dy)
+    assert int((dy0 != dy).sum()) <= max(4, z.numel() // 100)
+    ins = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = dense.linear(*ins, activation="relu")
+    within(y.detach(), want, slack)
+    y.backward(dy0)
+    for t, (grad, gslack) in zip(ins, grads64(x, w, dy0, slope, zs, "relu", DT[dt])):
+        within(t.grad, grad, gslack)
+    want, slack, parts = glu64(x, w, wu, "relu")
+    dy0 = torch.where(parts[0].abs() <= parts[1], torch.zeros_like(dy), dy)
+    assert int((dy0 != dy).sum()) <= max(4, z.numel() // 100)
+    ins = [t.clone().requires_grad_() for t in (x, w, wu)]
+    h = dense.glu(*ins, activation="relu")
+    within(h.detach(), want, slack)
+    h.backward(dy0)
+    for t, (grad, gslack) in zip(ins, glu_grads64(x, w, wu, dy0, parts, DT[dt])):
+        within(t.grad, grad, gslack)
