@@ -319,8 +319,8 @@ int64_t bcfft_dense_workspace_bytes(int op, int64_t n_tokens, int64_t in_feature
                                     int act);
 
 /* How one product of such a call is cut on the current device: *kind, the rows x columns of a workgroup's tile
- * (0: few rows, or few tokens' weight gradient; 1: 128 x 128; 2: 256 x 128; 3: 256 x 256; 4: 64 x 128; 5: 32 x
- * 128; 6: 64 x 64), and *slices of k. product: of a forward 0; of a backward 0 the input gradient, 1 the weight
+ * (0: few rows, or few tokens' weight gradient; 1: 128 x 128; 2: 256 x 128, 16 bits; 3: 256 x 256; 4: 64 x 128;
+ * 5: 32 x 128, fp32; 6: 64 x 64), and *slices of k. product: of a forward 0; of a backward 0 the input gradient, 1 the weight
  * gradient. Which calls run the same kernels, for tests and measurements; n_tokens >= 1. */
 int bcfft_dense_plan(int op, int product, int64_t n_tokens, int64_t in_features, int64_t out_features, int dtype, int* kind,
                      int* slices);

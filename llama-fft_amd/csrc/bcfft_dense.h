@@ -34,8 +34,9 @@ struct DzArgs {
   int act, rows;                         // rows per workgroup (dz)
 };
 
-// how a product is cut: tile kind (0: few rows or tokens, 1: 128 x 128, 2: 256 x 128, 3: 256 x 256, 4: 64 x 128, 5: 32 x
-// 128 with B by columns, 6: 64 x 64 but for the gated form) and slices of k
+// how a product is cut: tile kind (0: few rows or tokens, 1: 128 x 128, 2: 256 x 128 of 16 bits, 3: 256 x 256, 4: 64 x
+// 128 with A by rows, 5: 32 x 128 of fp32 with A by rows and B by columns, 6: 64 x 64 with A by rows but for the gated
+// form) and slices of k
 struct Shape {
   int kind, kz;
 };

@@ -130,7 +130,9 @@ __global__ __launch_bounds__(256) void bc_dense_pack_kernel(const char* __restri
 // Small tiles spread small products: 128 x 1024 -> 4096 takes 12.0 us in 128 x 128 tiles, 9.3 in 64 x 128, 7.4 in 64
 // x 64 (fp32 65.7, 36.8, 21.3); 1024 x 4096 -> 4096 43.3, 50.5, 65.3.
 // Few rows leave most of a 128-row tile's products empty, which fp32 pays for (4096 -> 4096, by columns: 20 rows
-// 38.6 us, 24.0 in 64-row tiles, 19.6 in 32-row tiles; bf16 13.1, 12.1, 11.5).
+// 38.6 us, 24.0 in 64-row tiles, 19.6 in 32-row tiles).
+// Not built: fp32 256 x 128 (two 128 x 128 tiles take 3.70 a step against 3.72) and 16-bit 32 x 128 (as many tiles as
+// 64 x 128, a step of 0.38 + 0.16 u against 0.37 + 0.09 u): the estimate never takes them.
 // Up to 32 rows run the few-rows kernel; more, 64 at a time, where that takes less than tiles with `pack`, the
 // packing of their operands: all of x passes through every CU that has a workgroup, 16 rows of W at a time
 // (16-bit 48 x 4096 -> 4096: 20.6 us against 16.8, with 4954 features, packed, 30.4 against 36.8; 512 x 512 -> 512
@@ -139,9 +141,9 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
   if (cols == 0 && m <= 32) return {0, 1};
   const int64_t cus = device_cu_count();
   struct Kind { int kind, bm, bn; double idle, busy, alone, fixed, step32, alone32, fixed32; };
-  const Kind kinds[6] = {{1, 128, 128, 0.30, 0.20, 0.12, 3.0, 1.85, 0.15, 4.7}, {2, 256, 128, 0.46, 0.40, 0.10, 3.0, 3.72, 0.0, 9.6},
+  const Kind kinds[6] = {{1, 128, 128, 0.30, 0.20, 0.12, 3.0, 1.85, 0.15, 4.7}, {2, 256, 128, 0.46, 0.40, 0.10, 3.0, 0.0, 0.0, 0.0},
                          {3, 256, 256, 0.90, 0.56, 0.06, 6.0, 7.3, 0.0, 16.0}, {4, 64, 128, 0.25, 0.09, 0.12, 2.0, 0.95, 0.12, 3.2},
-                         {5, 32, 128, 0.26, 0.16, 0.12, 2.5, 0.50, 0.45, 3.0}, {6, 64, 64, 0.16, 0.08, 0.19, 1.3, 0.47, 0.08, 2.5}};
+                         {5, 32, 128, 0.0, 0.0, 0.0, 0.0, 0.50, 0.45, 3.0}, {6, 64, 64, 0.16, 0.08, 0.19, 1.3, 0.47, 0.08, 2.5}};
   constexpr double START = 2.0;                        // of a tile launch beyond the few-rows kernel's
   Shape best{1, 1};
   double least = 1e300;
@@ -152,6 +154,7 @@ static Shape choose(int64_t m, int64_t n, int64_t ksteps, int parts, int dt, int
     best = {0, 1};
   }
   for (const Kind& q : kinds) {
+    if ((dt == BCFFT_F32 ? q.step32 : q.idle) == 0.0) continue;          // not built for the type
     if ((q.kind == 4 && cols == 2) || (q.kind == 5 && (cols != 1 || m > 32)) || (q.kind == 6 && (cols == 2 || parts == 2))) continue;
     const int64_t tiles = ((m + q.bm - 1) / q.bm) * ((n * parts + q.bn - 1) / q.bn);
     for (int64_t kz = 1; kz <= 16 && (kz == 1 || ksteps / kz >= 4); ++kz) {

@@ -244,16 +244,15 @@ static void launch_tile(const DenseArgs& a, hipStream_t s) {
 template <int DT, bool CA, bool CB, bool GLU>
 static void launch_tiles(const DenseArgs& a, int kind, hipStream_t s) {
   if (kind == 1) launch_tile<DT, CA, CB, 128, 128, 2, 2, 3, 2, GLU>(a, s);
-  else if (kind == 2) launch_tile<DT, CA, CB, 256, 128, 4, 2, 3, 3, GLU>(a, s);
-  else if (kind == 3) launch_tile<DT, CA, CB, 256, 256, 2, 4, 3, 2, GLU>(a, s);
-  else if constexpr (!CA) {
-    if (kind == 4) {
-      launch_tile<DT, CA, CB, 64, 128, 2, 2, 3, 3, GLU>(a, s);
-    } else if constexpr (!GLU) {
-      if (kind == 6) launch_tile<DT, CA, CB, 64, 64, 2, 2, 3, 3, GLU>(a, s);
-      else if constexpr (CB) launch_tile<DT, CA, CB, 32, 128, 1, 4, 3, 3, GLU>(a, s);
-    }
-  }
+  if constexpr (DT != BCFFT_F32)
+    if (kind == 2) launch_tile<DT, CA, CB, 256, 128, 4, 2, 3, 3, GLU>(a, s);
+  if (kind == 3) launch_tile<DT, CA, CB, 256, 256, 2, 4, 3, 2, GLU>(a, s);
+  if constexpr (!CA)
+    if (kind == 4) launch_tile<DT, CA, CB, 64, 128, 2, 2, 3, 3, GLU>(a, s);
+  if constexpr (DT == BCFFT_F32 && CB && !CA)
+    if (kind == 5) launch_tile<DT, CA, CB, 32, 128, 1, 4, 3, 3, GLU>(a, s);
+  if constexpr (!CA && !GLU)
+    if (kind == 6) launch_tile<DT, CA, CB, 64, 64, 2, 2, 3, 3, GLU>(a, s);
   if (a.kz > 1) {
     const int64_t quads = (a.n + 3) / 4 * a.m;
     const unsigned blocks = (unsigned)((quads + 255) / 256 < 16384 ? (quads + 255) / 256 : 16384);

@@ -40,6 +40,28 @@ def test_few_rows_sizes_run_the_few_rows_kernel(built_lib, gated, dtype):
     assert all(("forward", 0, False) in plans(gated, dtype, *s) for s in FEW_ROWS)
 
 
+# what is built, by product: kinds of tiles, split and unsplit (0: the few-rows / few-tokens kernels, unsplit)
+BUILT = {("forward", LINEAR): {F32: {1, 3, 4, 6}, SHORT: {1, 2, 3, 4, 6}},
+         ("forward", GLU): {F32: {1, 3, 4}, SHORT: {1, 2, 3, 4}},
+         ("input gradient", None): {F32: {1, 3, 4, 5, 6}, SHORT: {1, 2, 3, 4, 6}},
+         ("weight gradient", None): {F32: {1, 3}, SHORT: {1, 2, 3}}}
+
+
+@pytest.mark.parametrize("gated", [LINEAR, GLU])
+@pytest.mark.parametrize("dtype", [F32, SHORT])
+def test_every_kernel_that_is_built_is_reached(built_lib, gated, dtype):
+    """And no other is asked for: a kind that is not built would launch nothing."""
+    reached = set().union(*[plans(gated, dtype, *s) for s in VARIANTS[gated, dtype]])
+    anywhere = reached.union(*[plans(gated, dtype, *s) for s in sizes(4000, 8)])
+    for product in ("forward", "input gradient", "weight gradient"):
+        kinds = BUILT.get((product, gated), BUILT.get((product, None)))[dtype]
+        built = {(product, kind, split) for kind in kinds for split in (False, True)}
+        if product != "input gradient":
+            built.add((product, 0, False))
+        assert {p for p in reached if p[0] == product} == built
+        assert {p for p in anywhere if p[0] == product} == built
+
+
 def test_plan_refusals(built_lib):
     from bcfft import _lib
     lib, a, b = _lib.load(), ctypes.c_int(), ctypes.c_int()
