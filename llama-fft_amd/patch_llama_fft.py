@@ -480,67 +480,71 @@ def _hooks_on_every_module() -> bool:
                 m._global_backward_pre_hooks)
 
 
-def _plain_tensor(t: torch.Tensor) -> bool:
-    """Memory that a kernel can read, or a traced stand-in for it: a subclass (sharded, quantised) computes its
-    products itself."""
-    return type(t) in (torch.Tensor, nn.Parameter, torch._subclasses.FakeTensor)
+# memory that a kernel can read, or a traced stand-in for it: another subclass (sharded, quantised) computes its
+# products itself
+_FakeTensor = torch._subclasses.FakeTensor
+_PLAIN_TENSORS = (torch.Tensor, nn.Parameter, _FakeTensor)
 
 
-def _traced_gradient(*ts: torch.Tensor | None) -> bool:
+def _traced_gradient(*ts: torch.Tensor) -> bool:
     """A gradient is recorded while a tracer watches (torch.compile, FakeTensors, make_fx, any dispatch mode):
     the dense operators' autograd nodes launch kernels, which a trace does not hold."""
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)):
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in ts)):
         return False
     return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or any(type(t) is torch._subclasses.FakeTensor for t in ts))
+            or any(type(t) is _FakeTensor for t in ts))
 
 
-def _transformed(*ts: torch.Tensor | None) -> bool:
+def _transformed(*ts: torch.Tensor) -> bool:
     """Inside a torch.func transform, or dual tensors: the modules' products have rules for them. (torch.compile
     traces a transform's body apart from it; its view of the transforms' stack is not this thread's.)"""
     if not torch.compiler.is_compiling() and torch._C._functorch.peek_interpreter_stack() is not None:
         return True
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
-def _dense_mlp_sizes_ok(mlp, x: torch.Tensor) -> bool:
+def _dense_mlp_sizes_ok(x, w_gate, w_up, w_down) -> bool:
     """What bcfft.dense serves; a projection of other sizes than x's or than its neighbour's is its modules' to refuse."""
-    inner, hidden = mlp.gate_proj.weight.shape
-    return (mlp.up_proj.weight.shape == (inner, hidden) and x.dim() >= 1 and x.shape[-1] == hidden
+    (inner, hidden), (out, inner_down) = w_gate.shape, w_down.shape
+    shape = x.shape
+    return (w_up.shape == w_gate.shape and inner_down == inner and len(shape) >= 1 and shape[-1] == hidden
             and 1 <= hidden <= _dense.MAX_FEATURES and 1 <= inner <= _dense.MAX_FEATURES // 2
-            and mlp.down_proj.weight.shape[1] == inner and 1 <= mlp.down_proj.weight.shape[0] <= _dense.MAX_FEATURES
-            and x.numel() // hidden <= _dense.MAX_TOKENS)
+            and 1 <= out <= _dense.MAX_FEATURES and x.numel() // hidden <= _dense.MAX_TOKENS)
 
 
-def _dense_mlp_ok(mlp, x: torch.Tensor, residual: torch.Tensor | None) -> bool:
-    """The dense kernels take plain device tensors of one dtype, plain nn.Linear modules and SiLU; anything else
-    (autocast, tensor subclasses, a traced training step, torch.func transforms and dual tensors, sizes past the
-    kernels', a residual that broadcasts, a projection or the activation replaced later, hooks or a forward set
-    on one) runs the modules' own forward."""
-    mods = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
-    if not all(type(m) is nn.Linear for m in mods) or not _plain_silu(mlp.act_fn):
-        return False
-    if not all(_as_its_class(m) for m in (*mods, mlp.act_fn)) or _hooks_on_every_module():
-        return False
-    if mlp.gate_proj.bias is not None or mlp.up_proj.bias is not None or torch.is_autocast_enabled("cuda"):
-        return False
-    if not x.is_cuda or x.dtype not in _lib.DTYPE_CODE or not _dense_mlp_sizes_ok(mlp, x):
-        return False
-    if residual is not None and residual.shape != (*x.shape[:-1], mlp.down_proj.weight.shape[0]):
-        return False
-    ts = (x, mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight, mlp.down_proj.bias, residual)
-    return not _traced_gradient(*ts) and not _transformed(*ts) and all(
-        t is None or (_plain_tensor(t) and t.dtype == x.dtype and t.device == x.device) for t in ts)
+def _dense_mlp_operands(mlp, x: torch.Tensor, residual: torch.Tensor | None):
+    """The weights and down_proj's bias for the dense kernels, which take plain device tensors of one dtype, plain
+    nn.Linear modules and SiLU; None for anything else (autocast, tensor subclasses, a traced training step,
+    torch.func transforms and dual tensors, sizes past the kernels', a residual that broadcasts, a projection or
+    the activation replaced later, hooks or a forward set on one): the modules' own forward runs."""
+    gate, up, down, act = mlp.gate_proj, mlp.up_proj, mlp.down_proj, mlp.act_fn
+    if not (type(gate) is nn.Linear and type(up) is nn.Linear and type(down) is nn.Linear and _plain_silu(act)):
+        return None
+    if not (_as_its_class(gate) and _as_its_class(up) and _as_its_class(down) and _as_its_class(act)):
+        return None
+    dtype, device = x.dtype, x.device
+    if _hooks_on_every_module() or device.type != "cuda" or dtype not in _lib.DTYPE_CODE or torch.is_autocast_enabled("cuda"):
+        return None
+    ws = w_gate, w_up, w_down, bias = gate.weight, up.weight, down.weight, down.bias
+    if gate.bias is not None or up.bias is not None or not _dense_mlp_sizes_ok(x, w_gate, w_up, w_down):
+        return None
+    if residual is not None and residual.shape != (*x.shape[:-1], w_down.shape[0]):
+        return None
+    ts = [t for t in (x, *ws, residual) if t is not None]
+    if _traced_gradient(*ts) or _transformed(*ts):
+        return None
+    return ws if all(
+        type(t) in _PLAIN_TENSORS and t.dtype == dtype and t.device == device for t in ts) else None
 
 
 def _dense_mlp_forward(self, x, residual=None):
     """down(silu(gate(x)) * up(x)) (+ residual, in the down projection's epilogue) in two launches."""
-    if not _dense_mlp_ok(self, x, residual):
+    ws = _dense_mlp_operands(self, x, residual)
+    if ws is None:
         y = self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
         return y if residual is None else y + residual
-    h = _dense.glu(x, self.gate_proj.weight, self.up_proj.weight, activation="silu")
-    return _dense.linear(h, self.down_proj.weight, self.down_proj.bias, residual=residual)
+    w_gate, w_up, w_down, bias = ws
+    return _dense.linear(_dense.glu(x, w_gate, w_up, activation="silu"), w_down, bias, residual=residual)
 
 
 def fuse_dense_mlp(model) -> int:
