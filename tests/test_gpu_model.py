@@ -80,3 +80,34 @@ def test_model_bench_last_k_layers():
     assert cfg["patched_layers"] == 1 and cfg["fused_qkv_layers"] == 1 and cfg["fused_gate_up_layers"] == 1
     for name, r in line["projection_parity_first_patched_layer"].items():
         assert r["rel_err_vs_rounded"] < 1e-3, (name, r)
+
+
+def test_model_bench_compares_like_with_like():
+    """The MLPs that a patch leaves dense run the same kernels in the dense model and in the student: torch's, or with
+    --fuse-dense-mlp those of fuse_dense_mlp in both, the plain dense model's time beside them."""
+    pytest.importorskip("transformers")
+    import model_bench as MB
+    import patch_llama_fft as P
+    calls = []
+    fuse = P.fuse_dense_mlp
+
+    def watched(model):
+        calls.append(fuse(model))
+        return calls[-1]
+    args = ["--layers", "3", "--prompts", "4", "--max-len", "24", "--batch-size", "2", "--runs", "1", "--warmup", "0",
+            "--new-tokens", "0", "--num-layers", "1", "--config-overrides",
+            '{"hidden_size": 1024, "intermediate_size": 2816, "num_attention_heads": 8, "num_key_value_heads": 8, '
+            '"vocab_size": 512}']
+    try:
+        P.fuse_dense_mlp = watched
+        line = MB.main(args)
+        assert calls == [] and line["config"]["fused_dense_mlp_layers"] == 0 and "plain_dense_prefill_ms" not in line
+        line = MB.main(args + ["--fuse-dense-mlp", "1"])
+    finally:
+        P.fuse_dense_mlp = fuse
+    assert calls == [3, 2] and line["config"]["fused_dense_mlp_layers"] == 2
+    assert abs(line["bc_vs_dense_prefill"] - line["dense_prefill_ms"] / line["prefill_ms"]) < 2e-3 * line["bc_vs_dense_prefill"] + 1e-3
+    assert abs(line["bc_vs_plain_dense_prefill"] - line["plain_dense_prefill_ms"] / line["prefill_ms"]) < \
+        2e-3 * line["bc_vs_plain_dense_prefill"] + 1e-3
+    # the student's logits come from the same weights: the metrics stay what they are
+    assert line["teacher_student"]["last_topk_kl"] >= 0

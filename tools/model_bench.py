@@ -11,7 +11,9 @@ padded batches and model.generate. Here:
     metrics show the harness working, not LLaMA quality;
   * patch_linear_with_block_circulant (q/k/v/o/gate/up/down; --targets mlp for the reference's
     MLP-only patch), then fuse_attention_qkv and fuse_mlp_gate_up (one launch for q/k/v; the
-    whole MLP in one launch when all its projections are BC, else one for gate/up + SwiGLU);
+    whole MLP in one launch when all its projections are BC, else one for gate/up + SwiGLU).
+    bc_vs_dense_prefill compares models whose dense MLPs run the same kernels: torch's, or with
+    --fuse-dense-mlp 1 those of fuse_dense_mlp in both;
   * multi-GPU (config 5): one process per GPU under torch.distributed.run; each rank holds the
     whole model and takes a contiguous slice of the prompts (prompt-level replicas, no collective
     in the forward); at the end ONE all-gather (RCCL) of the last-token logits. Throughput is all
@@ -216,6 +218,9 @@ def main(argv=None):
     ap.add_argument("--runs", type=int, default=3)
     ap.add_argument("--new-tokens", type=int, default=32, help="greedy decode length (0: skip)")
     ap.add_argument("--dense", type=int, default=1, help="also time the dense (teacher) model's decode")
+    ap.add_argument("--fuse-dense-mlp", type=int, default=0,
+                    help="1: the dense MLPs of BOTH models run through fuse_dense_mlp (the dense model, and the "
+                         "layers that the patch leaves); the plain dense prefill is timed beside it")
     ap.add_argument("--topk", type=int, default=5)
     ap.add_argument("--temperature", type=float, default=1.0)
     ap.add_argument("--seed", type=int, default=0)
@@ -269,7 +274,11 @@ def main(argv=None):
     n_patch = cfg.num_hidden_layers if args.num_layers < 0 else args.num_layers
     patched = P._layer_indices(cfg.num_hidden_layers, n_patch, args.patch_position)
 
-    teacher_last, t_dense = prefill(model, batches, args.warmup, args.runs)
+    teacher_last, t_plain = prefill(model, batches, args.warmup, args.runs)
+    t_dense = t_plain
+    if args.fuse_dense_mlp:
+        P.fuse_dense_mlp(model)
+        t_dense = prefill(model, batches, args.warmup, args.runs)[1]
     dense_decode_s = decode(model, batches, args.new_tokens, cfg.pad_token_id) if args.dense and args.new_tokens else None
 
     line = None
@@ -288,7 +297,7 @@ def main(argv=None):
             patch(model, num_layers_to_patch=n_patch, block_size=b, patch_position=args.patch_position)
         n_qkv = P.fuse_attention_qkv(model)
         n_glu = P.fuse_mlp_gate_up(model)
-        n_dense = P.fuse_dense_mlp(model)                       # the MLPs the patch leaves dense
+        n_dense = P.fuse_dense_mlp(model) if args.fuse_dense_mlp else 0     # the MLPs the patch leaves dense
         torch.cuda.synchronize()
         res["patch_s"] = time.perf_counter() - t0
         torch.cuda.empty_cache()
@@ -340,6 +349,9 @@ def main(argv=None):
                 "teacher_student": metrics,
                 "projection_parity_first_patched_layer": parity,
             }
+            if args.fuse_dense_mlp:
+                line["plain_dense_prefill_ms"] = round(t_plain * 1e3, 3)
+                line["bc_vs_plain_dense_prefill"] = round(t_plain / t_bc, 3)
             if "bc_decode_s" in res:
                 line["decode_new_tokens_per_s"] = round(n_prompts_new / res["bc_decode_s"], 1)
             if dense_decode_s:
