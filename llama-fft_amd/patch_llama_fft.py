@@ -556,7 +556,6 @@ def fuse_dense_mlp(model) -> int:
     state_dict are unchanged; an MLP one of whose three projections, or whose activation, is replaced
     afterwards, holds hooks or a forward of its own runs as the modules that they are; an MLP whose instance
     already has a forward of another origin is left alone. Returns the number of MLPs rewired."""
-    import types
     n = 0
     for layer in model.model.layers:
         mlp = getattr(layer, "mlp", None)
@@ -568,9 +567,10 @@ def fuse_dense_mlp(model) -> int:
         if not _plain_silu(getattr(mlp, "act_fn", None)):
             continue
         forward = mlp.__dict__.get("forward")       # a wrapper around the MLP stays; this file's rewirings do not
-        if forward is not None and getattr(forward, "__func__", None) not in (_dense_mlp_forward, _fused_mlp_forward):
+        made_by = getattr(forward, "func", None) or getattr(forward, "__func__", None)
+        if forward is not None and made_by not in (_dense_mlp_forward, _fused_mlp_forward):
             continue
-        mlp.forward = types.MethodType(_dense_mlp_forward, mlp)
+        mlp.forward = functools.partial(_dense_mlp_forward, mlp)    # a bound method is not found when a saved model loads
         n += 1
     return n
 

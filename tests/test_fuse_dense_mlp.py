@@ -278,3 +278,22 @@ def test_transforms_run_the_modules(fake, fused_calls):
     assert t.shape == x.shape
     assert torch.func.vmap(mlp)(x).shape == x.shape
     assert fused_calls == ["glu", "linear"]
+
+
+def test_copies_and_saved_models_are_their_own():
+    """A copied or saved-and-loaded MLP runs its own weights, rewired as the original."""
+    import copy
+    import io
+    mlp = MLP(device="cpu", dtype=torch.float32)
+    x = torch.randn(2, HIDDEN)
+    want = mlp(x).detach()
+    assert P.fuse_dense_mlp(model_of(mlp)) == 1
+    file = io.BytesIO()
+    torch.save(mlp, file)
+    file.seek(0)
+    for other in (copy.deepcopy(mlp), torch.load(file, weights_only=False)):
+        assert torch.equal(other(x), want) and torch.equal(mlp(x), want)
+        with torch.no_grad():
+            other.down_proj.weight.zero_()
+        assert not bool(other(x).any()) and torch.equal(mlp(x), want)
+        assert "forward" in other.__dict__ and P.fuse_dense_mlp(model_of(other)) == 1
