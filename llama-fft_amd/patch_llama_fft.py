@@ -486,13 +486,14 @@ _FakeTensor = torch._subclasses.FakeTensor
 _PLAIN_TENSORS = (torch.Tensor, nn.Parameter, _FakeTensor)
 
 
-def _traced_gradient(*ts: torch.Tensor) -> bool:
-    """A gradient is recorded while a tracer watches (torch.compile, FakeTensors, make_fx, any dispatch mode):
-    the dense operators' autograd nodes launch kernels, which a trace does not hold."""
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in ts)):
+def _untraceable(*ts: torch.Tensor) -> bool:
+    """A tracer watches (torch.compile, FakeTensors, make_fx, any dispatch mode) a call that it cannot hold: one
+    that records a gradient (the dense operators' autograd nodes launch kernels), or one while the C++ operators
+    are not loaded (by the first call that is not traced; ctypes reads the tensors' memory)."""
+    if not (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or any(type(t) is _FakeTensor for t in ts)):
         return False
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or any(type(t) is _FakeTensor for t in ts))
+    return not _lib._native or (torch.is_grad_enabled() and any(t.requires_grad for t in ts))
 
 
 def _transformed(*ts: torch.Tensor) -> bool:
@@ -531,7 +532,7 @@ def _dense_mlp_operands(mlp, x: torch.Tensor, residual: torch.Tensor | None):
     if residual is not None and residual.shape != (*x.shape[:-1], w_down.shape[0]):
         return None
     ts = [t for t in (x, *ws, residual) if t is not None]
-    if _traced_gradient(*ts) or _transformed(*ts):
+    if _untraceable(*ts) or _transformed(*ts):
         return None
     return ws if all(
         type(t) in _PLAIN_TENSORS and t.dtype == dtype and t.device == device for t in ts) else None

@@ -31,7 +31,8 @@ def model_of(*mlps):
 @pytest.fixture
 def fused_calls(monkeypatch):
     """The calls of the dense operators, which stand in by their shapes."""
-    from bcfft import dense
+    from bcfft import _lib, dense
+    monkeypatch.setattr(_lib, "_native", True)
     calls = []
 
     def glu(x, w_gate, w_up, *, activation="silu"):
@@ -198,14 +199,14 @@ def test_traced_gradients_run_the_modules(fused_calls, monkeypatch):
 
     # the same decision for memory that is there, by the state of the tracer alone
     real = torch.empty(2, requires_grad=True)
-    assert not P._traced_gradient(real)
+    assert not P._untraceable(real)
     with monkeypatch.context() as mp:
         mp.setattr(torch.compiler, "is_compiling", lambda: True)
-        assert P._traced_gradient(real) and not P._traced_gradient(real.detach())
+        assert P._untraceable(real) and not P._untraceable(real.detach())
     with mode:
-        assert P._traced_gradient(real)
+        assert P._untraceable(real)
         with torch.no_grad():
-            assert not P._traced_gradient(real)
+            assert not P._untraceable(real)
 
 
 def test_sizes_past_the_operators_run_the_modules(fake, fused_calls):
@@ -297,3 +298,26 @@ def test_copies_and_saved_models_are_their_own():
             other.down_proj.weight.zero_()
         assert not bool(other(x).any()) and torch.equal(mlp(x), want)
         assert "forward" in other.__dict__ and P.fuse_dense_mlp(model_of(other)) == 1
+
+
+def test_compiled_before_any_call(built_lib, monkeypatch):
+    """The first call may be a traced one: until another has loaded the C++ operators, the modules are traced."""
+    from bcfft import _lib
+    if not _lib.native_op():
+        pytest.skip("the C++ operators are not built")
+    graphs = []
+
+    def backend(gm, inputs):
+        graphs.append([str(n.target) for n in gm.graph.nodes if n.op == "call_function"])
+        return gm
+
+    with FakeTensorMode(), torch.no_grad():
+        for loaded in (None, True, False):              # False: not built, or another engine library
+            monkeypatch.setattr(_lib, "_native", loaded)
+            torch._dynamo.reset()
+            graphs.clear()
+            mlp, x = rewired()
+            assert torch.compile(mlp, backend=backend, fullgraph=True)(x).shape == x.shape
+            ours = [g.split(".")[1] for g in graphs[0] if g.startswith("bcfft_native")]
+            assert len(graphs) == 1 and ours == (["dense_glu", "dense_linear"] if loaded else []), graphs
+            assert mlp(x).shape == x.shape             # FakeTensors without a compiler
