@@ -150,9 +150,9 @@ def load() -> ctypes.CDLL:
 def native_op() -> bool:
     """True once torch.ops.bcfft_native is loaded: the hot forward / forward_glu calls, the dense
     projections and the distillation operators then go through one C++ dispatcher op (argument checks,
-    allocation, stream lookup and the launch in C++) instead of ctypes. False when that library is not built, when BCFFT_NATIVE_OP=0, when
-    BCFFT_LIB_PATH names another engine library (the operators link the in-tree libbcfft.so), or
-    when the library is present but does not load (e.g. built against another torch: undefined
+    allocation, stream lookup and the launch in C++) instead of ctypes. False when that library is not
+    built, when BCFFT_NATIVE_OP=0, when BCFFT_LIB_PATH names another engine library (the operators link
+    the in-tree libbcfft.so), or when the library is present but does not load (e.g. built against another torch: undefined
     c10 symbols), which warns once. Either way the kernels are libbcfft.so's (the ctypes path
     calls the same ABI): there is no CPU path."""
     global _native, NATIVE_FORWARD, NATIVE_FORWARD_GLU

@@ -1,7 +1,7 @@
 // Further C++ torch operators over the C ABI (include/bcfft.h), in torch.ops.bcfft_native: the dense
 // projections and top-logit distillation with their autograd nodes. What bcfft/dense.py and bcfft/distill.py
 // do through ctypes and Python autograd Functions (170 us of host time for a forward and backward), in one
-// dispatcher call and a C++ node each. Same checks, errors and semantics as the Python path, which stays as
+// dispatcher call and a C++ node each (27-95 us by operator and host). Same checks, errors and semantics as the Python path, which stays as
 // the fallback when this library is not built. Host code only: the kernels are libbcfft.so's.
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
